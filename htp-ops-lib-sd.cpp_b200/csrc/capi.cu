@@ -21,6 +21,7 @@
 #include "../../include/htp_ops_b200.h"
 #include "../../include/op_reg.h"
 #include "kernels.h"
+#include "ops.h"
 #include "scratch_run.h"
 
 using namespace htpg;
@@ -50,6 +51,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
 struct Workspace {
   void *base = nullptr;
   size_t bytes = 0;
+  bool captured = false;  // ows: a captured graph may refer to the block
 };
 
 struct Device {
@@ -59,6 +61,7 @@ struct Device {
   uint32_t *watchdog = nullptr;
   std::map<cudaStream_t, Workspace> ws;
   std::map<cudaStream_t, Workspace> qws;  // opcodes 2-4: counters | partials | FP16 operands
+  std::map<cudaStream_t, Workspace> ows;  // block operators: counters | partials
   cudaEvent_t ev[4] = {nullptr, nullptr, nullptr, nullptr};
 };
 
@@ -84,10 +87,11 @@ int current_device(Device **out) {
   return HTPG_OK;
 }
 
-// Zero every stream workspace of the device (W8A8/FP16 split-K areas and the
-// opcode 2-4 stream-K scratch); the device is idle when this is called.
+// Zero every stream workspace of the device (W8A8/FP16 split-K areas, the
+// opcode 2-4 stream-K scratch, the block operators' counters); the device is
+// idle when this is called.
 void clear_workspaces(Device *d) {
-  for (auto *m : {&d->ws, &d->qws})
+  for (auto *m : {&d->ws, &d->qws, &d->ows})
     for (auto &kv : *m)
       if (kv.second.base && cudaMemset(kv.second.base, 0, kv.second.bytes) != cudaSuccess) cudaGetLastError();
   cudaDeviceSynchronize();
@@ -294,7 +298,7 @@ extern "C" int htpg_debug_simulate_abort(uint32_t fill) {
   int rc = current_device(&d);
   if (rc) return rc;
   if (cudaDeviceSynchronize() != cudaSuccess) return record_cuda(cudaGetLastError());
-  for (auto *m : {&d->ws, &d->qws})
+  for (auto *m : {&d->ws, &d->qws, &d->ows})
     for (auto &kv : *m)
       if (kv.second.base && cudaMemset(kv.second.base, static_cast<int>(fill & 0xffu), kv.second.bytes) != cudaSuccess)
         return record_cuda(cudaGetLastError());
@@ -1112,6 +1116,80 @@ extern "C" int htpg_f16_linear(float *out, const float *x, const uint16_t *permu
   if (rc) return rc;
   return run_common(w, &out, 1, 0, x, bias, m, channels, mode, stream);
 }
+
+// ================================================================ block operators
+namespace htpg {
+
+int op_device(OpDevice *out) {
+  Device *d;
+  const int rc = current_device(&d);
+  if (rc) return rc;
+  out->sms = d->sms;
+  out->watchdog = d->watchdog;
+  return HTPG_OK;
+}
+
+int op_result(cudaError_t e) { return record_cuda(e); }
+
+std::unique_lock<std::mutex> op_lock() { return std::unique_lock<std::mutex>(g_mu); }
+
+int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return HTPG_ELAUNCH;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) return record_cuda(cudaGetLastError());
+  Workspace &w = g_dev[dev].ows[st];
+  const size_t need = kOpCounters * sizeof(uint32_t) + bytes;
+  if (w.bytes < need) {
+    if (cap != cudaStreamCaptureStatusNone) {
+      t_last_cuda_error = "the stream's scratch would have to grow during capture: run the call once before";
+      return HTPG_ENOMEM;
+    }
+    const size_t want = align_up(need + need / 4, 1u << 20);
+    void *base = nullptr;
+    if (cudaMalloc(&base, want) != cudaSuccess) {
+      cudaGetLastError();
+      return HTPG_ENOMEM;
+    }
+    if (cudaMemsetAsync(base, 0, want, st) != cudaSuccess) {
+      const int rc = record_cuda(cudaGetLastError());
+      cudaFree(base);
+      return rc;
+    }
+    if (w.base && !w.captured) {
+      cudaStreamSynchronize(st);
+      cudaFree(w.base);
+    }
+    w.base = base;
+    w.bytes = want;
+    w.captured = false;
+  }
+  if (cap != cudaStreamCaptureStatusNone) w.captured = true;
+  *counters = static_cast<uint32_t *>(w.base);
+  *scratch = static_cast<uint8_t *>(w.base) + kOpCounters * sizeof(uint32_t);
+  return HTPG_OK;
+}
+
+int op_tensor_map(CUtensorMap *map, int type, const void *base, const uint64_t (&dims)[4],
+                  const uint64_t (&strides)[3], const uint32_t (&box)[4]) {
+  if (!g_encode) return HTPG_ELAUNCH;
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) d[i] = dims[i], b[i] = box[i];
+  for (int i = 0; i < 3; ++i) s[i] = strides[i];
+  const CUresult r = g_encode(map,
+                              type == HTPG_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                              4, const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    t_last_cuda_error = "cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")";
+    return HTPG_ELAUNCH;
+  }
+  return HTPG_OK;
+}
+
+}  // namespace htpg
 
 // ================================================================ opcodes 2-4
 namespace {

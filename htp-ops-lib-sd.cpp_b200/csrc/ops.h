@@ -1,0 +1,84 @@
+// Shared by the transformer-block operators (rope.cu, attention.cu, lora.cu):
+// the library's device state, stream scratch and launches, and element types.
+// Internal to libhtp_ops_b200.so.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+
+#include "../../include/htp_ops_b200.h"
+#include "kernels.h"
+
+namespace htpg {
+
+// ---- device state (capi.cu)
+struct OpDevice {
+  int sms = 0;
+  uint32_t *watchdog = nullptr;
+};
+// The current device, initialised when this is its first use.
+int op_device(OpDevice *d);
+// Text for htpg_last_cuda_error; HTPG_OK or HTPG_ELAUNCH.
+int op_result(cudaError_t e);
+// The library's lock: held from op_scratch to the launch that uses the scratch,
+// so that no other host thread grows (moves) it in between.
+std::unique_lock<std::mutex> op_lock();
+// Scratch of one stream: `bytes` of it, preceded by kOpCounters zero words that
+// every launch leaves zero.  Grows when a larger call arrives (not while the
+// stream is being captured: HTPG_ENOMEM) and is kept otherwise; a block that a
+// captured graph may refer to is never freed.
+constexpr int kOpCounters = 16384;
+int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch);
+// Tensor map of a 16-bit array of up to 4 dimensions (innermost first; strides
+// in bytes of dimensions 1 .. 3), zero fill, 128-byte swizzle.
+int op_tensor_map(CUtensorMap *map, int type, const void *base, const uint64_t (&dims)[4],
+                  const uint64_t (&strides)[3], const uint32_t (&box)[4]);
+
+// Launch as a programmatic dependent: the kernel waits (grid_dependency_wait)
+// before it touches memory, so only its set-up overlaps the kernel before it.
+template <typename... P, typename... A>
+cudaError_t op_launch(void (*fn)(P...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return counted(cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...));
+}
+
+// ---- element types
+inline int type_bytes(int type) {
+  return type == HTPG_TYPE_F32 ? 4 : type == HTPG_TYPE_F16 || type == HTPG_TYPE_BF16 ? 2 : 0;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  if constexpr (sizeof(T) == 4)
+    return v;
+  else if constexpr (std::is_same<T, __half>::value)
+    return __half2float(v);
+  else
+    return __bfloat162float(v);
+}
+// Round to nearest even.
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+  if constexpr (sizeof(T) == 4)
+    return v;
+  else if constexpr (std::is_same<T, __half>::value)
+    return __float2half_rn(v);
+  else
+    return __float2bfloat16_rn(v);
+}
+
+}  // namespace htpg

@@ -21,6 +21,10 @@ OK, EPAYLOAD, EUNMAPPED, EHEADER = 0, -1, -2, -3
 EARGS, ECAPACITY, ECONTROL, ELAUNCH, ENOPLAN = -10, -11, -12, -13, -14
 EWATCHDOG, ENOMEM, ESCRATCH, EARCH = -16, -17, -18, -75
 BUF_DEVICE, BUF_HOST = 0, 1
+# element types (ggml numbers)
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 
 _lib = None
 
@@ -123,6 +127,10 @@ def lib() -> ctypes.CDLL:
         "htpg_qk0_run": (I, [P, P, P, I, P]),
         "htpg_qk0_dequantize": (I, [P, P, I, I, I, P]),
         "htpg_qk0_plan_info": (I, [I, I, I, I, I, ctypes.POINTER(I64)]),
+        "htpg_rope_table": (I, [P, I, I, P, P]),
+        "htpg_qkv_rope": (I, [P] * 12),
+        "htpg_cross_attention": (I, [P] * 8),
+        "htpg_lora_run": (I, [P] * 10),
         "htp_ops_open": (I, [ctypes.c_char_p, ctypes.POINTER(U64)]),
         "htp_ops_close": (I, [U64]),
         "htp_ops_init_backend": (I, [U64]),
@@ -425,3 +433,127 @@ def aux_params_bytes(prm: dict, eps: float = 1e-6, output=(-1, 0), input_=(-1, 0
     import struct
     return (struct.pack("<8i", *output, *input_, *weight, *bias) +
             struct.pack("<9i", *[prm[f] for f in AUX_FIELDS]) + struct.pack("<fi", eps, 0))
+
+
+# ------------------------------------------------------------------ transformer block operators
+# Per-head norm and rotation, cross attention and low-rank adapters.  Each call
+# takes a parameter block (sizes, types, strides) built once from its tensors
+# and the tensors' addresses of this call; it returns the library's code.
+class RopeScaling(ctypes.Structure):
+    """struct htpg_rope_scaling."""
+    _fields_ = [("scaling", ctypes.c_int32), ("original_rows", ctypes.c_int32), ("base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double)]
+
+
+class RopeParams(ctypes.Structure):
+    """struct htpg_rope_params."""
+    _fields_ = [(f, ctypes.c_int32) for f in ("in_type", "out_type", "batch", "seq", "q_heads", "kv_heads",
+                                              "head_dim", "rot_dim", "layout", "table_rows")] + \
+               [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)] + \
+               [(f, ctypes.c_int64 * 3) for f in ("q_stride", "k_stride", "v_stride", "q_out_stride",
+                                                  "k_out_stride", "v_out_stride")]
+
+
+class AttentionParams(ctypes.Structure):
+    """struct htpg_attention_params."""
+    _fields_ = [(f, ctypes.c_int32) for f in ("type", "out_type", "batch", "q_len", "kv_len", "q_heads", "kv_heads",
+                                              "head_dim")] + \
+               [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] + \
+               [(f, ctypes.c_int64 * 3) for f in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
+               [("bias_stride", ctypes.c_int64)]
+
+
+class LoraParams(ctypes.Structure):
+    """struct htpg_lora_params."""
+    _fields_ = [(f, ctypes.c_int32) for f in ("type", "m", "k", "n", "adapters", "max_rank")] + \
+               [(f, ctypes.c_int64) for f in ("ldx", "ldb", "ldo")]
+
+
+def type_of(t) -> int:
+    """HTPG_TYPE_* of a torch tensor."""
+    import torch
+    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    if t.dtype not in types:
+        raise ValueError(f"no library type for {t.dtype}")
+    return types[t.dtype]
+
+
+def _strides(t):
+    """{batch, token, head} strides of a [batch][tokens][heads][dim] tensor; None: zeros."""
+    if t is None:
+        return (0, 0, 0)
+    if t.dim() != 4 or (t.stride(3) != 1 and t.shape[3] > 1):
+        raise ValueError("expected [batch][tokens][heads][dim] with contiguous dim")
+    return t.stride()[:3]
+
+
+def rope_table(table, rot_dim: int, scaling: int = ROPE_PLAIN, base: float = 10000.0, factor: float = 1.0,
+               original_rows: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0, stream=None) -> int:
+    """Fill table [rows][rot_dim / 2][2] (FP32) with cosines and sines of rotary positions."""
+    s = RopeScaling(scaling, original_rows, base, factor, beta_fast, beta_slow)
+    return lib().htpg_rope_table(ptr(table), table.shape[0], rot_dim, ctypes.byref(s), stream_ptr(stream))
+
+
+def rope_params(q, k, v, q_out, k_out, v_out, rot_dim: int, layout: int, table_rows: int,
+                eps: float = 1e-6) -> RopeParams:
+    """Parameters of qkv_rope from its [batch][seq][heads][dim] tensors (pairs that are None are left out)."""
+    parts = [(i, o) for i, o in ((q, q_out), (k, k_out), (v, v_out)) if i is not None]
+    if not parts or any((i is None) != (o is None) for i, o in ((q, q_out), (k, k_out), (v, v_out))):
+        raise ValueError("q, k and v are each given with their output or left out with it")
+    first, out = parts[0]
+    kv = k if k is not None else v
+    for i, o in parts:
+        if i.shape != o.shape or i.dtype != first.dtype or o.dtype != out.dtype or i.shape[:2] != first.shape[:2] or \
+                i.shape[3] != first.shape[3]:
+            raise ValueError("q, k, v and their outputs differ in batch, tokens, dim or type")
+    if k is not None and v is not None and k.shape != v.shape:
+        raise ValueError("k and v differ in shape")
+    p = RopeParams(type_of(first), type_of(out), first.shape[0], first.shape[1],
+                   q.shape[2] if q is not None else 0, kv.shape[2] if kv is not None else 0, first.shape[3], rot_dim,
+                   layout, table_rows, eps, 0)
+    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out), ("v_out", v_out)):
+        getattr(p, name + "_stride")[:] = _strides(t)
+    return p
+
+
+def qkv_rope(prm: RopeParams, q_out, k_out, v_out, q, k, v, q_weight=None, k_weight=None, table=None,
+             positions=None, stream=None) -> int:
+    return lib().htpg_qkv_rope(ctypes.byref(prm), ptr(q_out), ptr(k_out), ptr(v_out), ptr(q), ptr(k), ptr(v),
+                               ptr(q_weight), ptr(k_weight), ptr(table), ptr(positions), stream_ptr(stream))
+
+
+def attention_params(out, q, k, v, scale: float, bias_stride: int | None = None) -> AttentionParams:
+    """Parameters of cross_attention from its [batch][tokens][heads][dim] tensors; bias_stride: elements between
+    the key bias's rows (default: kv_len)."""
+    if out.shape != q.shape or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or \
+            k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k, v and out differ in shape or type")
+    p = AttentionParams(type_of(q), type_of(out), q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2],
+                        q.shape[3], scale, 0)
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        getattr(p, name + "_stride")[:] = _strides(t)
+    p.bias_stride = k.shape[1] if bias_stride is None else bias_stride
+    return p
+
+
+def cross_attention(prm: AttentionParams, out, q, k, v, kv_lens=None, key_bias=None, stream=None) -> int:
+    return lib().htpg_cross_attention(ctypes.byref(prm), ptr(out), ptr(q), ptr(k), ptr(v), ptr(kv_lens),
+                                      ptr(key_bias), stream_ptr(stream))
+
+
+def lora_params(out, base, x, a, b) -> LoraParams:
+    """Parameters of lora_run: x [m][k], out and base [m][n] FP32, a [adapters][max_rank][k], b [adapters][n][max_rank]."""
+    if a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.dtype != b.dtype or a.shape[2] != x.shape[1] or \
+            b.shape[1] != out.shape[1] or x.shape[0] != out.shape[0] or (base is not None and base.shape != out.shape):
+        raise ValueError("x, a, b, base and out do not fit together")
+    if not (a.is_contiguous() and b.is_contiguous()):
+        raise ValueError("a and b are dense")
+    if any(t is not None and t.stride(1) != 1 for t in (x, base, out)):
+        raise ValueError("rows of x, base and out are contiguous")
+    return LoraParams(type_of(a), x.shape[0], x.shape[1], out.shape[1], a.shape[0], a.shape[1], x.stride(0),
+                      base.stride(0) if base is not None else 0, out.stride(0))
+
+
+def lora_run(prm: LoraParams, out, base, x, row_adapter, a, b, ranks, scales, stream=None) -> int:
+    return lib().htpg_lora_run(ctypes.byref(prm), ptr(out), ptr(base), ptr(x), ptr(row_adapter), ptr(a), ptr(b),
+                               ptr(ranks), ptr(scales), stream_ptr(stream))

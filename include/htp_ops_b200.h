@@ -192,6 +192,135 @@ int htpg_qk0_plan_info(int weight_type, int m, int n, int k, int sms, int64_t ou
  * htpg_set_qdec_shape does not fit. */
 int htpg_qk0_decode_plan_info(int weight_type, int m, int n, int k, int sms, int64_t out[8]);
 
+/* ---- operators of a text-conditioned transformer block -------------------
+ * (no counterpart in the reference's linear path)
+ *
+ * Element types, by their ggml numbers. */
+#define HTPG_TYPE_F32 0
+#define HTPG_TYPE_F16 1
+#define HTPG_TYPE_BF16 30
+
+/* Cosines and sines of rotary positions: table[rows][rot_dim / 2][2] (FP32,
+ * cos then sin) of position p = 0 .. rows - 1 and pair i, computed in FP64 as
+ * p * f_i with f_i = base^(-2i / rot_dim), adapted to a context longer than
+ * the trained one by `scaling`:
+ *   HTPG_ROPE_PLAIN   as is
+ *   HTPG_ROPE_LINEAR  f_i / factor (positions interpolated)
+ *   HTPG_ROPE_NTK     base * factor^(rot_dim / (rot_dim - 2)) (rot_dim > 2)
+ *   HTPG_ROPE_YARN    f_i (1 - r) + f_i / factor * r, with the ramp r =
+ *                     clamp((i - low) / (high - low), 0, 1) from the pair that
+ *                     turns beta_fast times over original_rows to the one that
+ *                     turns beta_slow times: low = max(floor(c(beta_fast)), 0),
+ *                     high = min(ceil(c(beta_slow)), rot_dim - 1) (low + 0.001
+ *                     when not above low), c(t) = rot_dim / 2 *
+ *                     ln(original_rows / (2 pi t)) / ln(base); cos and sin are
+ *                     multiplied by 0.1 ln(factor) + 1
+ * rot_dim even, >= 2; base > 1; factor >= 1. */
+#define HTPG_ROPE_PLAIN 0
+#define HTPG_ROPE_LINEAR 1
+#define HTPG_ROPE_NTK 2
+#define HTPG_ROPE_YARN 3
+struct htpg_rope_scaling {
+  int32_t scaling;
+  int32_t original_rows;         /* YARN: the trained context length */
+  double base;                   /* e.g. 10000 */
+  double factor;                 /* how many times longer the context is */
+  double beta_fast, beta_slow;   /* YARN: e.g. 32 and 1 */
+};
+int htpg_rope_table(float *table, int rows, int rot_dim, const struct htpg_rope_scaling *scaling, void *stream);
+
+/* Per-head RMS norm and rotary positions of projected queries and keys, and
+ * the conversion of the values, in one pass over the projection's output.
+ * Per row (batch, token, head) of q and k:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight[d]     (x where weight is NULL)
+ * then the first rot_dim elements are rotated in pairs (a, b) by the table
+ * row of the token's position: a' = a cos - b sin, b' = a sin + b cos.  Pair i
+ * is elements (2i, 2i + 1) with HTPG_ROPE_INTERLEAVED and (i, i + rot_dim / 2)
+ * with HTPG_ROPE_HALF.  Elements past rot_dim are only normed; v is only
+ * converted.  The arithmetic is FP32, rounded once at the store.
+ *
+ * Tensors are [batch][seq][heads][head_dim] with element strides {batch,
+ * token, head} and contiguous head_dim: the q, k and v columns of one packed
+ * projection, [batch][heads][seq][head_dim] outputs and the like.  q with
+ * q_out, k with k_out and v with v_out are each given or both NULL.  positions:
+ * [batch][seq] int32 device array of table rows, or NULL for the token's index
+ * in its sequence.  A position outside [0, table_rows) reads nothing and makes
+ * its q and k rows NaN.  An output may be its own input (equal types and strides);
+ * otherwise outputs overlap nothing.  table: 8-byte aligned; weights FP32
+ * [head_dim].  head_dim <= 512; batch or seq 0: nothing is done. */
+#define HTPG_ROPE_INTERLEAVED 0
+#define HTPG_ROPE_HALF 1
+struct htpg_rope_params {
+  int32_t in_type, out_type; /* HTPG_TYPE_* */
+  int32_t batch, seq;
+  int32_t q_heads, kv_heads, head_dim;
+  int32_t rot_dim; /* even, 0 .. head_dim; 0: no rotation (table NULL) */
+  int32_t layout;
+  int32_t table_rows;
+  float eps;
+  int32_t reserved; /* 0 */
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t q_out_stride[3], k_out_stride[3], v_out_stride[3];
+};
+int htpg_qkv_rope(const struct htpg_rope_params *p, void *q_out, void *k_out, void *v_out, const void *q,
+                  const void *k, const void *v, const float *q_weight, const float *k_weight, const float *table,
+                  const int32_t *positions, void *stream);
+
+/* Attention of q_len query tokens over an encoder's kv_len states (no causal
+ * mask), softmax in FP32:
+ *   out[b][i][h] = sum_j w_j v[b][j][h'] / sum_j w_j,
+ *   w_j = exp(scale * q[b][i][h] . k[b][j][h'] + key_bias[b][j]),
+ * h' = h / (q_heads / kv_heads).  Only keys j < kv_lens[b] (clamped to [0,
+ * kv_len]; NULL: kv_len) whose bias is not -inf take part: whatever K and V
+ * hold at the others, infinities and NaN included, changes nothing.  A row
+ * with no such key is zero.  key_bias: FP32 [batch][kv_len] (row stride
+ * bias_stride elements, 0 shares one row), or NULL.
+ *
+ * q, out: [batch][q_len][q_heads][head_dim]; k, v: [batch][kv_len][kv_heads]
+ * [head_dim]; element strides {batch, token, head}, contiguous head_dim; batch
+ * stride 0 in k and v shares one encoder's states.  type: F16 or BF16 (q, k,
+ * v); out_type: the same or F32.  The weights are rounded to `type` for the
+ * product with V; with an F32 output they are carried in two parts (twice the
+ * bits), so that the result is good to about 2^-21 (F16) or 2^-16 (BF16) of
+ * the values.  head_dim: a multiple of 8 up to 192; q_heads a multiple of
+ * kv_heads; scale > 0; pointers 16-byte aligned and q, k, v strides multiples
+ * of 8 elements (out: 16 bytes) (HTPG_ECONTROL).  batch or q_len 0: nothing is
+ * done; kv_len 0: zeros. */
+struct htpg_attention_params {
+  int32_t type, out_type; /* HTPG_TYPE_* */
+  int32_t batch, q_len, kv_len;
+  int32_t q_heads, kv_heads, head_dim;
+  float scale;
+  int32_t reserved; /* 0 */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  int64_t bias_stride;
+};
+int htpg_cross_attention(const struct htpg_attention_params *p, void *out, const void *q, const void *k,
+                         const void *v, const int32_t *kv_lens, const float *key_bias, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[i] = base[i] + scales[s] * (x[i] A_s^T) B_s^T,   s = row_adapter[i],
+ * with A_s the first ranks[s] rows of a[s] ([adapters][max_rank][k]) and B_s
+ * the first ranks[s] columns of b[s] ([adapters][n][max_rank]).  Rows whose
+ * row_adapter is outside [0, adapters) get base[i].  What a and b hold past an
+ * adapter's rank is not read into the result; ranks are clamped to [0,
+ * max_rank].  base may be out (the projection's output, added to in place) or
+ * NULL (zeros).  All of row_adapter [m], ranks and scales [adapters] (int32,
+ * int32, FP32) are device arrays.  x, base, out FP32 with row strides ldx, ldb,
+ * ldo (0: dense); a, b of `type` (F16 or BF16).  FP32 accuracy: x and the
+ * intermediate x A^T are split so that no bits that FP32 keeps are lost.
+ * k, n: multiples of 8; max_rank: a multiple of 8 up to 128; pointers 16-byte
+ * aligned, ld* multiples of 4 (HTPG_ECONTROL).  m = 0: nothing is done. */
+struct htpg_lora_params {
+  int32_t type; /* of a and b */
+  int32_t m, k, n;
+  int32_t adapters, max_rank;
+  int64_t ldx, ldb, ldo;
+};
+int htpg_lora_run(const struct htpg_lora_params *p, float *out, const float *base, const float *x,
+                  const int32_t *row_adapter, const void *a, const void *b, const int32_t *ranks,
+                  const float *scales, void *stream);
+
 /* ---- column-sharded run with a fused output exchange -------------------- */
 /* Multi-GPU form of htpg_w8a8_run for a weight split by output columns (N)
  * across ranks, each rank holding a column block: the epilogue stores every
