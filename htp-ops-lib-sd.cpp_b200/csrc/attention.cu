@@ -3,6 +3,7 @@
 //   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i . k_j + bias_j)
 //
 // in one pass over the keys with the running maximum and sum of the softmax.
+#include <algorithm>
 #include <cmath>
 #include <exception>
 
@@ -88,10 +89,569 @@ cudaError_t launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
   return op_launch(attn_row_kernel<T, TO>, dim3(grid), kRowWarps * 32, 0, st, a);
 }
 
-// 16-byte vectors along every dimension that is stepped along.
+// ------------------------------------------------------------ tiles of rows
+// 128 query rows of one head are one tile: S = Q K^T (128 rows x up to KT keys)
+// and O += P V are tcgen05.mma into TMEM, softmax in registers, one thread per
+// row.  A CTA holds two tiles that share their keys and values (neighbouring
+// rows of one head, or heads of one group), so that the tensor core works for
+// one while the other's softmax runs:
+//   warps 0-3, 4-7  softmax of tile 0, 1: S from TMEM, running maximum and sum,
+//                   P (16 bits) back into TMEM over S, and the tile's output
+//   warp 8          issues the MMAs, warp 9 the TMA loads (10 and 11 only make
+//                   the warpgroup whole, to hand its registers to the others:
+//                   256 x 216 + 128 x 72 = 384 x 168, what the launch gives)
+// TMEM columns: S of tile 0 and 1 (KT each, P in place), O of both (DP each).
+// P is the A operand in TMEM; V, as loaded ([key][dim]), the MN-major B operand.
+// The maximum is only raised (and O rescaled) once a score passes it by 2^8:
+// weights up to 2^8 (FP16: 2^15, see kShift) stay exact enough and most tiles
+// skip the rescale.
+constexpr int kTileThreads = 384;
+constexpr int kLensHeld = 256;   // batches whose lengths are kept in shared memory
+constexpr float kLazy = 8.0f;    // log2 of how far a score may pass the held maximum
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct TileArgs {
+  AttnArgs a;
+  int row_tiles;       // 128-row tiles of one head
+  int pairs;           // tile pairs of one key/value head: ceil(group * row_tiles / 2)
+  int kv_heads;
+  int splits;          // ranges of keys of one pair
+  long long items;     // batch * kv_heads * pairs * splits
+  int q_batch, k_batch, k_head, v_batch, v_head;  // 0: that dimension's stride is 0 (one copy)
+  int wide;            // output rows are 32-byte aligned
+  float *part_o;       // splits > 1: [splits][rows][dim] sums
+  float2 *part_ml;     //             [splits][rows] maximum (log2) and sum
+  long long rows;
+  uint32_t *watchdog;
+};
+
+template <int DP, int KT>
+struct TileSmem {
+  static constexpr int kQ = 128 * DP * 2;
+  static constexpr int kStage = KT * DP * 2;
+  static constexpr int kStages = DP == 128 ? 4 : DP == 64 ? 6 : 5;
+  static constexpr int kBars = 2 * kQ + kStages * kStage;
+  static constexpr int kLens = kBars + 8 * (2 + 2 * kStages + 7) + 24;
+  static constexpr int kBias = (kLens + 4 * kLensHeld + 15) / 16 * 16;  // [tile][2][KT]
+  static constexpr int kBytes = kBias + 16 * KT + 1024;                 // + alignment
+};
+
+struct TileItem {
+  int b, kvh, n, j0, j1, split;  // n keys take part, tiles [j0, j1) of them are this item's
+  int head[2], row0[2];
+  bool two;
+};
+
+__device__ __forceinline__ int clamped_len(const AttnArgs &a, int b) {
+  return a.lens ? min(max(a.lens[b], 0), a.kv_len) : a.kv_len;
+}
+
+template <int KT>
+__device__ __forceinline__ TileItem tile_item(const TileArgs &t, long long item, const int *lens) {
+  TileItem r;
+  r.split = static_cast<int>(item % t.splits);
+  long long u = item / t.splits;
+  const int pair = static_cast<int>(u % t.pairs);
+  u /= t.pairs;
+  r.kvh = static_cast<int>(u % t.kv_heads);
+  r.b = static_cast<int>(u / t.kv_heads);
+  r.n = r.b < kLensHeld ? lens[r.b] : clamped_len(t.a, r.b);
+  const int tiles = (r.n + KT - 1) / KT, per = (tiles + t.splits - 1) / t.splits;
+  r.j0 = min(r.split * per, tiles);
+  r.j1 = min(r.j0 + per, tiles);
+  r.two = 2 * pair + 1 < t.a.group * t.row_tiles;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int tile = 2 * pair + w;
+    r.head[w] = r.kvh * t.a.group + tile / t.row_tiles;
+    r.row0[w] = tile % t.row_tiles * 128;
+  }
+  return r;
+}
+
+// Two FP32 values as one 16-bit pair (the first in the low half), to nearest even.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+__device__ __forceinline__ void store32(void *p, const uint32_t (&v)[8], bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4 *>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// 32 output columns [c, c + 32) of one row, those below dim.
+template <typename TO>
+__device__ __forceinline__ void store_columns(TO *row, int c, int dim, const float (&o)[32], bool wide) {
+  if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      if (c + j >= dim) break;
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[j + i]);
+      store32(row + c + j, v, wide);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j += 16) {
+      if (c + j >= dim) break;
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = pack2<TO>(o[j + 2 * i], o[j + 2 * i + 1]);
+      if (c + j + 16 <= dim)
+        store32(row + c + j, v, wide);
+      else
+        *reinterpret_cast<uint4 *>(row + c + j) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+template <typename T, typename TO, int DP, int KT>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TileArgs t) {
+  using L = TileSmem<DP, KT>;
+  // FP32 outputs: P in two 16-bit parts, high and low, each KT / 2 TMEM columns
+  constexpr bool kParts = sizeof(TO) == 4;
+  // FP16 weights are 2^7 times larger, so that those below 2^-14 of the
+  // largest keep their bits; with kLazy they stay below 2^15
+  constexpr float kShift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+  constexpr uint32_t kFormat = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr uint32_t kIdesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | (8u << 24);  // F32 sums, M = 128
+  constexpr int NS = L::kStages;
+  constexpr uint32_t kO = 2 * KT;  // first TMEM column of O
+
+  extern __shared__ uint8_t raw[];
+  uint8_t *base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t q_s = smem_u32(base), kv_s = q_s + 2 * L::kQ;
+  const uint32_t bars = q_s + L::kBars;
+  const uint32_t kv_full = bars, kv_empty = bars + 8 * NS, q_full = bars + 16 * NS, q_empty = q_full + 8;
+  const uint32_t s_full = q_empty + 8, p_ready = s_full + 16, o_full = p_ready + 16, mma_done = o_full + 16;
+  uint32_t *slot = reinterpret_cast<uint32_t *>(base + L::kBars + 8 * (2 * NS + 9));
+  volatile uint32_t *abort = slot + 1;
+  int *lens = reinterpret_cast<int *>(base + L::kLens);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    *abort = 0;
+    for (int i = 0; i < NS; ++i) mbar_init(kv_full + 8 * i, 1), mbar_init(kv_empty + 8 * i, 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full + 8 * w, 1);
+      mbar_init(p_ready + 8 * w, 4);
+      mbar_init(o_full + 8 * w, 1);
+    }
+    mbar_init(mma_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(slot), 512);
+    tmem_relinquish();
+  }
+  if (warp == 9 && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  grid_dependency_wait();
+  for (int i = threadIdx.x; i < min(t.a.batch, kLensHeld); i += kTileThreads) lens[i] = clamped_len(t.a, i);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  const int dim = t.a.dim;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 9 && lane == 0) {
+      // ------------------------------------------------------------ loads
+      bool ok = true;
+      uint32_t loads = 0, tiles = 0;  // K and V tiles, query tile pairs issued
+      auto load = [&](const CUtensorMap *map, int j, int h, int b) {
+        const uint32_t s = loads % NS, ph = loads / NS & 1u;
+        if (!mbar_wait(kv_empty + 8 * s, ph ^ 1u, t.watchdog, kWatchProducer, abort)) return false;
+        mbar_arrive_expect_tx(kv_full + 8 * s, ((dim + 63) / 64) * KT * 128);
+        for (int p = 0; p * 64 < dim; ++p)
+          tma_load_4d(kv_s + s * L::kStage + p * KT * 128, map, kv_full + 8 * s, p * 64, j * KT, h, b);
+        ++loads;
+        return true;
+      };
+      for (long long item = blockIdx.x; ok && item < t.items; item += gridDim.x) {
+        const TileItem it = tile_item<KT>(t, item, lens);
+        if (it.j0 == it.j1) continue;
+        ok = mbar_wait(q_empty, (tiles & 1u) ^ 1u, t.watchdog, kWatchProducer, abort);
+        if (!ok) break;
+        const int panels = (dim + 63) / 64;
+        mbar_arrive_expect_tx(q_full, (it.two ? 2 : 1) * panels * 128 * 128);
+        for (int w = 0; w < (it.two ? 2 : 1); ++w)
+          for (int p = 0; p < panels; ++p)
+            tma_load_4d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full, p * 64, it.row0[w], it.head[w], it.b * t.q_batch);
+        ++tiles;
+        for (int j = it.j0; ok && j < it.j1; ++j) {
+          ok = load(&map_k, j, it.kvh * t.k_head, it.b * t.k_batch);
+          ok = ok && load(&map_v, j, it.kvh * t.v_head, it.b * t.v_batch);
+        }
+      }
+      // never leave the CTA with a copy still landing in its shared memory
+      for (uint32_t i = loads > NS ? loads - NS : 0; i < loads; ++i)
+        mbar_wait(kv_full + 8 * (i % NS), i / NS & 1u, t.watchdog, kWatchProducer, abort);
+      if (tiles) mbar_wait(q_full, (tiles - 1) & 1u, t.watchdog, kWatchProducer, abort);
+    }
+    if (warp == 8 && lane == 0) {
+      // ------------------------------------------------------------- MMAs
+      bool ok = true;
+      uint32_t used = 0, tiles = 0, ready[2] = {0, 0};
+      const int ksteps = (dim + 15) / 16;
+      const uint32_t idesc_v = kIdesc | (1u << 16) | (static_cast<uint32_t>(ksteps * 2) << 17);  // V: MN-major, N = dim
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        const bool got = mbar_wait(bar, parity, t.watchdog, kWatchMma, abort);
+        tc_fence_after();
+        return got;
+      };
+      // S of tile w = Q K^T with the key tile in slot `u`
+      auto scores = [&](int w, uint32_t u, int keys) {
+        const uint32_t k_at = kv_s + (u % NS) * L::kStage, q_at = q_s + w * L::kQ;
+        const uint32_t idesc = kIdesc | (static_cast<uint32_t>((keys + 15) / 16 * 2) << 17);
+        for (int i = 0; i < ksteps; ++i)
+          umma_f16(tmem + w * KT, umma_desc_sw128(q_at + i / 4 * 128 * 128 + i % 4 * 32),
+                   umma_desc_sw128(k_at + i / 4 * KT * 128 + i % 4 * 32), idesc, i > 0);
+        tc_commit(s_full + 8 * w);
+      };
+      for (long long item = blockIdx.x; ok && item < t.items; item += gridDim.x) {
+        const TileItem it = tile_item<KT>(t, item, lens);
+        const int nt = it.j1 - it.j0, nw = it.two ? 2 : 1;
+        if (!nt) continue;
+        ok = wait(q_full, tiles & 1u) && wait(kv_full + 8 * (used % NS), used / NS & 1u);
+        if (!ok) break;
+        ++tiles;
+        for (int w = 0; w < nw; ++w) scores(w, used, min(KT, it.n - it.j0 * KT));
+        tc_commit(kv_empty + 8 * (used % NS));
+        if (nt == 1) tc_commit(q_empty);
+        for (int j = 0; ok && j < nt; ++j) {
+          // slots: key tile j = used, value tile j = used + 1, key tile j + 1 = used + 2
+          const int keys = min(KT, it.n - (it.j0 + j) * KT);
+          const uint32_t v_slot = (used + 1) % NS;
+          for (int w = 0; ok && w < nw; ++w) {
+            ok = wait(p_ready + 8 * w, ready[w]++ & 1u);
+            if (ok && w == 0) ok = wait(kv_full + 8 * v_slot, (used + 1) / NS & 1u);
+            if (!ok) break;
+            const int vsteps = (keys + 15) / 16;
+            for (int part = 0; part < (kParts ? 2 : 1); ++part)
+              for (int i = 0; i < vsteps; ++i)
+                umma_f16_ta(tmem + kO + w * DP, tmem + w * KT + part * (KT / 2) + i * 8,
+                            umma_desc_sw128_mn(kv_s + v_slot * L::kStage + i * 2048, KT * 128), idesc_v,
+                            j > 0 || part > 0 || i > 0);
+            if (w == nw - 1) tc_commit(kv_empty + 8 * v_slot);
+            if (j + 1 < nt) {
+              if (w == 0) ok = wait(kv_full + 8 * ((used + 2) % NS), (used + 2) / NS & 1u);
+              if (!ok) break;
+              scores(w, used + 2, min(KT, it.n - (it.j0 + j + 1) * KT));
+              if (w == nw - 1) {
+                tc_commit(kv_empty + 8 * ((used + 2) % NS));
+                if (j + 2 == nt) tc_commit(q_empty);
+              }
+            } else {
+              tc_commit(o_full + 8 * w);
+            }
+          }
+          used += 2;
+        }
+      }
+      tc_commit(mma_done);  // every MMA is complete before TMEM is freed
+      mbar_wait(mma_done, 0, t.watchdog, kWatchMma, abort);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int w = warp >> 2, quad = warp & 3, r = quad * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t s_at = tmem + w * KT + (static_cast<uint32_t>(quad) << 21);
+    const uint32_t o_at = tmem + kO + w * DP + (static_cast<uint32_t>(quad) << 21);
+    const float c = t.a.scale * kLog2e;
+    const bool wide = t.wide != 0;
+    float *bias_s = reinterpret_cast<float *>(base + L::kBias) + w * 2 * KT;
+    uint32_t seen = 0, done = 0, used = 0;
+    bool ok = true;
+    auto wait = [&](bool go, uint32_t bar, uint32_t parity) {
+      const bool got = go && mbar_wait(bar, parity, t.watchdog, kWatchEpilogue, abort);
+      tc_fence_after();
+      return __all_sync(0xffffffffu, got) != 0;
+    };
+    // No early exit: a tile's threads meet at its named barriers in every
+    // iteration; after a wait that gave up they skip the work.
+    for (long long item = blockIdx.x; item < t.items; item += gridDim.x) {
+      const TileItem it = tile_item<KT>(t, item, lens);
+      const int nt = it.j1 - it.j0;
+      if (w == 1 && !it.two) {
+        used += 2 * nt;
+        continue;
+      }
+      const bool mine = it.row0[w] + r < t.a.q_len;
+      const float *bias = t.a.bias ? t.a.bias + it.b * t.a.bias_stride : nullptr;
+      const float unit = bias ? 1.0f : c;  // of the scores in s[], in log2
+      float top = -INFINITY, sum = 0.0f;
+      for (int j = 0; j < nt; ++j, used += 2) {
+        const int k0 = (it.j0 + j) * KT, keys = min(KT, it.n - k0);
+        bool dead = r < KT && r >= keys;
+        if (bias) {
+          // one key per thread: in units of log2, the lowest finite bias kept
+          // finite; two buffers, so that one barrier a tile is enough
+          float add = r < keys ? ld_dep(bias + k0 + r) : -INFINITY;
+          dead = r < KT && add == -INFINITY;
+          if (!dead) add = fmaxf(add * kLog2e, -3.402823466e38f);
+          if (r < KT) bias_s[(j & 1) * KT + r] = add;
+          named_bar_sync(1 + w, 128);
+        }
+        ok = wait(ok, s_full + 8 * w, seen++ & 1u);
+        if (!ok) continue;
+        float s[KT / 32][32];
+#pragma unroll
+        for (int g = 0; g < KT / 32; ++g)
+          if (g * 32 < keys) tmem_ld32(s_at + g * 32, s[g]);
+        tmem_ld_wait();
+        // what takes no part becomes -inf; with a bias scores are in units of log2
+        if (bias) {
+          const float *add = bias_s + (j & 1) * KT;
+#pragma unroll
+          for (int i = 0; i < KT; ++i) {
+            const float x = add[i];
+            s[i / 32][i % 32] = x == -INFINITY ? -INFINITY : fmaf(s[i / 32][i % 32], c, x);
+          }
+        } else if (keys < KT) {
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+            if (i >= keys) s[i / 32][i % 32] = -INFINITY;
+        }
+        float most = s[0][0];
+#pragma unroll
+        for (int i = 1; i < KT; ++i) most = fmaxf(most, s[i / 32][i % 32]);
+        most *= unit;
+        const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float keep = raise ? ex2_approx(top - most) : 1.0f;
+          if (raise) {
+            top = most;
+            sum *= keep;
+          }
+          if (j > 0) {
+            // the tensor core is done with O: S of this tile came after it
+#pragma unroll
+            for (int i = 0; i < DP; i += 32) {
+              if (i < dim) {
+                uint32_t o[32];
+                tmem_ld32(o_at + i, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                tmem_st32(o_at + i, o);
+              }
+            }
+          }
+        }
+        const float from = top == -INFINITY ? 0.0f : top - kShift;
+#pragma unroll
+        for (int g = 0; g < KT / 32; ++g) {
+          if (g * 32 < keys) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const float p0 = ex2_approx(fmaf(s[g][2 * x], unit, -from));
+              const float p1 = ex2_approx(fmaf(s[g][2 * x + 1], unit, -from));
+              sum += p0;
+              sum += p1;
+              hi[x] = pack2<T>(p0, p1);
+              if (kParts) {
+                const float2 back = unpack2<T>(hi[x]);
+                lo[x] = pack2<T>(p0 - back.x, p1 - back.y);
+              }
+            }
+            tmem_st16(s_at + g * 16, hi);
+            if (kParts) tmem_st16(s_at + KT / 2 + g * 16, lo);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        // Values of keys that take no part may be infinite or NaN, which a
+        // zero weight would not remove: tile 0's threads, one key each, clear
+        // them before the first product that reads them.
+        if (w == 0 && (bias || it.n < t.a.kv_len)) {
+          dead = dead && r < (keys + 15) / 16 * 16;
+          if (__any_sync(0xffffffffu, dead)) {
+            const uint32_t v_slot = (used + 1) % NS;
+            ok = wait(ok, kv_full + 8 * v_slot, (used + 1) / NS & 1u);
+            if (!ok) continue;
+            if (dead)
+              for (int p = 0; p * 64 < dim; ++p)
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                  *reinterpret_cast<uint4 *>(base + 2 * L::kQ + v_slot * L::kStage + p * KT * 128 + r * 128 + x * 16) =
+                      make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + 8 * w);
+      }
+      if (nt) ok = wait(ok, o_full + 8 * w, done++ & 1u);
+      if (!ok) continue;
+      const float inv = t.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+      const bool none = sum == 0.0f;
+      const long long row = (static_cast<long long>(it.b) * t.a.q_heads + it.head[w]) * t.a.q_len + it.row0[w] + r;
+      TO *out = static_cast<TO *>(t.a.out) + it.b * t.a.os[0] + static_cast<long long>(it.row0[w] + r) * t.a.os[1] +
+                it.head[w] * t.a.os[2];
+      float *part = t.splits > 1 ? t.part_o + (it.split * t.rows + row) * dim : nullptr;
+#pragma unroll
+      for (int i = 0; i < DP; i += 32) {
+        if (i < dim) {
+          float o[32];
+          if (nt) {
+            tmem_ld32(o_at + i, o);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = none ? 0.0f : o[x] * inv;
+          if (mine) {
+            if (part)
+              store_columns<float>(part, i, dim, o, true);
+            else
+              store_columns<TO>(out, i, dim, o, wide);
+          }
+        }
+      }
+      if (part && mine) t.part_ml[it.split * t.rows + row] = make_float2(none ? -INFINITY : top, sum);
+      tc_fence_before();  // O has been read before the next tile's P is announced
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the key ranges of each row in order: one warp per row.
+template <typename TO>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ TileArgs t) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= t.rows) return;
+  float top = -INFINITY;
+  for (int s = 0; s < t.splits; ++s) top = fmaxf(top, t.part_ml[s * t.rows + row].x);
+  const float from = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  for (int s = 0; s < t.splits; ++s) {
+    const float2 ml = t.part_ml[s * t.rows + row];
+    sum += ml.y * ex2_approx(ml.x - from);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const long long i = row % t.a.q_len, h = row / t.a.q_len % t.a.q_heads, b = row / t.a.q_len / t.a.q_heads;
+  TO *out = static_cast<TO *>(t.a.out) + b * t.a.os[0] + i * t.a.os[1] + h * t.a.os[2];
+  for (int d = lane; d < t.a.dim; d += 32) {
+    float o = 0.0f;
+    for (int s = 0; s < t.splits; ++s)
+      o += t.part_o[(s * t.rows + row) * t.a.dim + d] * ex2_approx(t.part_ml[s * t.rows + row].x - from);
+    out[d] = from_f32<TO>(sum == 0.0f ? 0.0f : o * inv);
+  }
+}
+// A 4-D map {dim, tokens, heads, batch} of one operand, boxes of 64 x box_rows.
+// Heads or batches that share one copy (stride 0) become one; strides of
+// extents of one are not looked at.
+int operand_map(CUtensorMap *map, int type, const void *base, int dim, int tokens, int heads, int batch,
+                const int64_t *stride, int box_rows, int *head_step, int *batch_step) {
+  *head_step = heads > 1 && stride[2] != 0;
+  *batch_step = batch > 1 && stride[0] != 0;
+  const uint64_t row = static_cast<uint64_t>(dim) * 2;
+  const uint64_t dims[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(tokens),
+                            static_cast<uint64_t>(*head_step ? heads : 1), static_cast<uint64_t>(*batch_step ? batch : 1)};
+  const uint64_t strides[3] = {tokens > 1 ? static_cast<uint64_t>(stride[1]) * 2 : row,
+                               *head_step ? static_cast<uint64_t>(stride[2]) * 2 : row,
+                               *batch_step ? static_cast<uint64_t>(stride[0]) * 2 : row};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
+  return op_tensor_map(map, type, base, dims, strides, box);
+}
+
+template <typename T, typename TO, int DP, int KT>
+int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const OpDevice &d, cudaStream_t st) {
+  TileArgs t = {};
+  t.a = a;
+  t.row_tiles = (a.q_len + 127) / 128;
+  t.kv_heads = p->kv_heads;
+  const long long pairs = (static_cast<long long>(a.group) * t.row_tiles + 1) / 2;
+  if (pairs > 0x3fffffff) return HTPG_ECAPACITY;
+  t.pairs = static_cast<int>(pairs);
+  t.rows = static_cast<long long>(a.batch) * a.q_heads * a.q_len;
+  t.watchdog = d.watchdog;
+  const long long units = pairs * t.kv_heads * a.batch;
+  const int tiles = (a.kv_len + KT - 1) / KT;
+  t.splits = 1;
+  if (units * 2 <= d.sms && tiles >= 4) t.splits = static_cast<int>(std::min<long long>(d.sms / units, tiles / 2));
+  t.items = units * t.splits;
+  t.wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
+  const int qe[3] = {a.batch, a.q_len, a.q_heads};
+  for (int i = 0; i < 3; ++i)
+    if (qe[i] > 1 && a.os[i] * sizeof(TO) % 32) t.wide = 0;
+  CUtensorMap mq, mk, mv;
+  int q_head, rc;
+  // a query head or token stride of 0 needs no map of its own: refused by the caller
+  if ((rc = operand_map(&mq, p->type, a.q, a.dim, a.q_len, a.q_heads, a.batch, p->q_stride, 128, &q_head, &t.q_batch)) ||
+      (rc = operand_map(&mk, p->type, a.k, a.dim, a.kv_len, p->kv_heads, a.batch, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
+      (rc = operand_map(&mv, p->type, a.v, a.dim, a.kv_len, p->kv_heads, a.batch, p->v_stride, KT, &t.v_head, &t.v_batch)))
+    return rc;
+  std::unique_lock<std::mutex> lock;
+  if (t.splits > 1) {
+    lock = op_lock();
+    uint32_t *counters;
+    uint8_t *scratch;
+    const size_t ml = (static_cast<size_t>(t.splits) * t.rows * sizeof(float2) + 255) / 256 * 256;
+    rc = op_scratch(st, ml + static_cast<size_t>(t.splits) * t.rows * a.dim * 4, &counters, &scratch);
+    if (rc) return rc;
+    t.part_ml = reinterpret_cast<float2 *>(scratch);
+    t.part_o = reinterpret_cast<float *>(scratch + ml);
+  }
+  auto *fn = attn_tile_kernel<T, TO, DP, KT>;
+  using L = TileSmem<DP, KT>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  if (e != cudaSuccess) return op_result(e);
+  e = op_launch(fn, dim3(static_cast<unsigned>(std::min<long long>(t.items, d.sms))), kTileThreads, L::kBytes, st, mq, mk,
+                mv, t);
+  if (e == cudaSuccess && t.splits > 1)
+    e = op_launch(attn_join_kernel<TO>, dim3(static_cast<unsigned>((t.rows + 7) / 8)), 256, 0, st, t);
+  return op_result(e);
+}
+
+template <typename T, typename TO>
+int run_attention(const struct htpg_attention_params *p, const AttnArgs &a, const OpDevice &d, cudaStream_t st) {
+  if (a.q_len <= 16 || a.kv_len == 0) return op_result(launch_attn<T, TO>(a, d.sms, st));
+  if (a.dim <= 64) return run_tiles<T, TO, 64, 128>(p, a, d, st);
+  if (a.dim <= 128) return run_tiles<T, TO, 128, 128>(p, a, d, st);
+  return run_tiles<T, TO, 192, 64>(p, a, d, st);
+}
+
+// 16-byte vectors along every dimension that is stepped along, forwards, and
+// within a tensor map's reach; tokens have rows of their own.
 bool strides_fit(const int64_t *s, const int (&extent)[3], int per16) {
   for (int i = 0; i < 3; ++i)
-    if (extent[i] > 1 && s[i] % per16) return false;
+    if (extent[i] > 1 && (s[i] % per16 || s[i] < (i == 1) || s[i] >= (int64_t{1} << 38))) return false;
   return true;
 }
 
@@ -143,11 +703,13 @@ extern "C" int htpg_cross_attention(const struct htpg_attention_params *p, void 
   a.dim = p->head_dim;
   a.scale = p->scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
-  if (p->type == HTPG_TYPE_F16)
-    e = p->out_type == HTPG_TYPE_F32 ? launch_attn<__half, float>(a, d.sms, st) : launch_attn<__half, __half>(a, d.sms, st);
-  else
-    e = p->out_type == HTPG_TYPE_F32 ? launch_attn<__nv_bfloat16, float>(a, d.sms, st)
-                                     : launch_attn<__nv_bfloat16, __nv_bfloat16>(a, d.sms, st);
-  return op_result(e);
+  try {
+    if (p->type == HTPG_TYPE_F16)
+      return p->out_type == HTPG_TYPE_F32 ? run_attention<__half, float>(p, a, d, st)
+                                          : run_attention<__half, __half>(p, a, d, st);
+    return p->out_type == HTPG_TYPE_F32 ? run_attention<__nv_bfloat16, float>(p, a, d, st)
+                                        : run_attention<__nv_bfloat16, __nv_bfloat16>(p, a, d, st);
+  } catch (const std::exception &) {
+    return HTPG_ENOMEM;
+  }
 }
