@@ -169,22 +169,6 @@ __device__ __forceinline__ TileItem tile_item(const TileArgs &t, long long item,
   return r;
 }
 
-// Two FP32 values as one 16-bit pair (the first in the low half), to nearest even.
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __half>::value)
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
-
 __device__ __forceinline__ void store32(void *p, const uint32_t (&v)[8], bool wide) {
   if (wide) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),

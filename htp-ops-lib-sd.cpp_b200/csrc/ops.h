@@ -10,6 +10,7 @@
 
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/htp_ops_b200.h"
 #include "kernels.h"
@@ -79,6 +80,22 @@ __device__ __forceinline__ T from_f32(float v) {
     return __float2half_rn(v);
   else
     return __float2bfloat16_rn(v);
+}
+
+// Two FP32 values as one 16-bit pair (the first in the low half), to nearest even.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
 }  // namespace htpg

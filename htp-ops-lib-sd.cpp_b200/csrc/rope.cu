@@ -6,8 +6,8 @@
 //
 // Every element is read and written once and does some ten operations, so the
 // pass is bound by HBM: (in + out) bytes per element.
+#include <algorithm>
 #include <cmath>
-#include <new>
 
 #include "ops.h"
 #include "ptx.cuh"
@@ -52,12 +52,13 @@ struct RopeArgs {
   const int *positions;
   int batch, seq, dim, rot, half, table_rows;
   int heads;  // of all parts
-  float eps;
+  float eps, inv_dim;
 };
 
 constexpr int kRopeWarps = 8, kRopeMaxDim = 512;
 
-// One warp per (token, head) row, the row staged in shared memory as FP32.
+// Any size and alignment (odd head dims, rotations that are no multiple of 4):
+// one warp per (token, head) row, the row staged in shared memory as FP32.
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_row_kernel(RopeArgs a) {
   __shared__ float rows[kRopeWarps][kRopeMaxDim];
@@ -108,9 +109,229 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_row_kernel(RopeArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- vectors
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+  return reinterpret_cast<float2 &>(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
+  return reinterpret_cast<float2 &>(r);
+}
+// N consecutive elements as FP32 (ONCE: evicted first), and back.
+template <typename T, int N, bool ONCE = true>
+__device__ __forceinline__ void load_n(const T *p, float *v) {
+  auto get = [](auto *q) { return ONCE ? __ldcs(q) : *q; };
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 x = get(reinterpret_cast<const float4 *>(p + i));
+        v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+      }
+    } else {
+      const float2 x = get(reinterpret_cast<const float2 *>(p));
+      v[0] = x.x, v[1] = x.y;
+    }
+  } else {
+    uint32_t r[(N + 1) / 2];
+    if constexpr (N == 8) {
+      const uint4 x = get(reinterpret_cast<const uint4 *>(p));
+      r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
+    } else if constexpr (N == 4) {
+      const uint2 x = get(reinterpret_cast<const uint2 *>(p));
+      r[0] = x.x, r[1] = x.y;
+    } else {
+      r[0] = get(reinterpret_cast<const uint32_t *>(p));
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 x = unpack2<T>(r[i / 2]);
+      v[i] = x.x, v[i + 1] = x.y;
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T *p, const float *v) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+      *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+    }
+  } else {
+    uint32_t r[(N + 1) / 2];
+#pragma unroll
+    for (int i = 0; i < N; i += 2) r[i / 2] = pack2<T>(v[i], v[i + 1]);
+    if constexpr (N == 8)
+      *reinterpret_cast<uint4 *>(p) = make_uint4(r[0], r[1], r[2], r[3]);
+    else if constexpr (N == 4)
+      *reinterpret_cast<uint2 *>(p) = make_uint2(r[0], r[1]);
+    else
+      *reinterpret_cast<uint32_t *>(p) = r[0];
+  }
+}
+
+// A row is dim / (2 W) slots of W pairs, one per lane of a group of 2^log_g
+// lanes: both halves' W elements (half layout) or 2 W neighbours (interleaved,
+// and past rot in both).  A group takes kHeads neighbouring heads of one part
+// of one token: their loads are all in flight together, with the lane's
+// weights, cosines and sines, which they share.  Nothing is staged: partners sit
+// in the same thread, and the norm is log_g shuffles.
+// HBM-bound once the instructions are few: part, heads and batch come from the
+// block's index (with one flat index, divided per thread, 212 instructions per
+// 8 elements left the pass issue-bound: 4.8 TB/s), and products are packed
+// pairs.  16384 tokens of 36 heads x 128, FP32 to FP16, cold L2: 80 us = 5.7
+// TB/s with two heads per group (one: 92; four: 82; six: 94; 16 elements per
+// lane and part: 80, but 104 against 88 with interleaved pairs).
+constexpr int kHeads = 2;
+template <typename TI, typename TO, bool HALF, int W>
+__global__ void __launch_bounds__(256) rope_vec_kernel(const __grid_constant__ RopeArgs a, int log_g) {
+  constexpr int U = kHeads;
+  grid_dependency_wait();
+  const unsigned g = 1u << log_g, slot = threadIdx.x & (g - 1);
+  // blocks: x tokens of one sequence, y a part's U heads, z the batch
+  const unsigned i = blockIdx.x * (blockDim.x >> log_g) + (threadIdx.x >> log_g), b = blockIdx.z;
+  if (i >= static_cast<unsigned>(a.seq)) return;  // whole groups; `mask` names the group alone
+  const unsigned mask = g == 32 ? 0xffffffffu : ((1u << g) - 1) << ((threadIdx.x & 31) & ~(g - 1));
+  const int per_q = (a.part[0].heads + U - 1) / U, per_k = (a.part[1].heads + U - 1) / U;
+  int h0 = blockIdx.y;
+  const int which = h0 < per_q ? 0 : h0 < per_q + per_k ? 1 : 2;
+  h0 = (h0 - (which > 0 ? per_q : 0) - (which > 1 ? per_k : 0)) * U;
+  const RopePart &p = a.part[which];
+  const bool live = slot * 2 * W < static_cast<unsigned>(a.dim);
+  const int rot = p.rotate ? a.rot : 0;
+  const bool turns = slot * 2 * W < static_cast<unsigned>(rot);
+  // offsets of the slot's two W-element parts
+  const int o0 = HALF && turns ? W * slot : 2 * W * slot, o1 = HALF && turns ? rot / 2 + W * slot : o0 + W;
+
+  const TI *in0 = static_cast<const TI *>(p.in) + b * p.in_stride[0] + i * p.in_stride[1] + h0 * p.in_stride[2];
+  float x[U][2 * W], w[2 * W];
+  float2 cs[W];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int e = 0; e < 2 * W; ++e) x[u][e] = 0.0f;
+    const TI *in = in0 + u * p.in_stride[2];
+    if (!live || h0 + u >= p.heads) continue;
+    if (HALF) {
+      load_n<TI, W>(in + o0, x[u]);
+      load_n<TI, W>(in + o1, x[u] + W);
+    } else {
+      load_n<TI, 2 * W>(in + o0, x[u]);
+    }
+  }
+  bool inside = true;
+  if (rot) {
+    const int pos = a.positions ? a.positions[static_cast<long long>(b) * a.seq + i] : static_cast<int>(i);
+    inside = pos >= 0 && pos < a.table_rows;
+    if (inside && turns) {
+      const float4 *t = reinterpret_cast<const float4 *>(a.table + static_cast<long long>(pos) * (rot / 2) + W * slot);
+#pragma unroll
+      for (int e = 0; e < W; e += 2) {
+        const float4 v = t[e / 2];
+        cs[e] = make_float2(v.x, v.y), cs[e + 1] = make_float2(v.z, v.w);
+      }
+    }
+  }
+  if (p.weight && live) {
+    load_n<float, W, false>(p.weight + o0, w);
+    load_n<float, W, false>(p.weight + o1, w + W);
+  }
+  float2 cos2[W / 2], sin2[W / 2], neg2[W / 2];  // of two neighbouring pairs
+#pragma unroll
+  for (int e = 0; e < W / 2; ++e) {
+    cos2[e] = make_float2(cs[2 * e].x, cs[2 * e + 1].x);
+    sin2[e] = make_float2(cs[2 * e].y, cs[2 * e + 1].y);
+    neg2[e] = make_float2(-sin2[e].x, -sin2[e].y);
+  }
+  TO *out = static_cast<TO *>(p.out) + b * p.out_stride[0] + i * p.out_stride[1] + h0 * p.out_stride[2];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (p.weight) {
+      float2 sq = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int e = 0; e < 2 * W; e += 2) {
+        const float2 v = make_float2(x[u][e], x[u][e + 1]);
+        sq = fma2(v, v, sq);
+      }
+      float sum = sq.x + sq.y;
+      for (unsigned o = g / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+      const float inv = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
+#pragma unroll
+      for (int e = 0; e < 2 * W; e += 2) {
+        const float2 v = mul2(mul2(make_float2(x[u][e], x[u][e + 1]), make_float2(inv, inv)), make_float2(w[e], w[e + 1]));
+        x[u][e] = v.x, x[u][e + 1] = v.y;
+      }
+    }
+    if (!live || h0 + u >= p.heads) continue;
+    if (turns) {
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) {
+        const int e0 = HALF ? 2 * e : 4 * e, e1 = HALF ? 2 * e + 1 : 4 * e + 2;  // first elements of two pairs
+        const int f0 = HALF ? W + e0 : e0 + 1, f1 = HALF ? W + e1 : e1 + 1;      // their second ones
+        const float2 p0 = make_float2(x[u][e0], x[u][e1]), p1 = make_float2(x[u][f0], x[u][f1]);
+        const float2 q0 = fma2(p1, neg2[e], mul2(p0, cos2[e])), q1 = fma2(p1, cos2[e], mul2(p0, sin2[e]));
+        x[u][e0] = q0.x, x[u][e1] = q0.y, x[u][f0] = q1.x, x[u][f1] = q1.y;
+      }
+    }
+    if (!inside) {
+#pragma unroll
+      for (int e = 0; e < 2 * W; ++e) x[u][e] = __int_as_float(0x7fffffff);
+    }
+    if (HALF) {
+      store_n<TO, W>(out + u * p.out_stride[2] + o0, x[u]);
+      store_n<TO, W>(out + u * p.out_stride[2] + o1, x[u] + W);
+    } else {
+      store_n<TO, 2 * W>(out + u * p.out_stride[2] + o0, x[u]);
+    }
+  }
+}
+
+// Whether every vector of the W-pair kernel is aligned, and a row fits one warp.
+bool vectors_fit(const RopeArgs &a, int w, int in_bytes, int out_bytes) {
+  if (a.dim % (2 * w) || a.rot % (2 * w) || a.dim / (2 * w) > 32) return false;
+  const int elements = a.half ? w : 2 * w;
+  const uintptr_t in_vec = std::min(16, elements * in_bytes), out_vec = std::min(16, elements * out_bytes);
+  if (reinterpret_cast<uintptr_t>(a.table) % 16) return false;
+  const int extent[3] = {a.batch, a.seq, 0};
+  for (const RopePart &p : a.part) {
+    if (!p.heads) continue;
+    if (reinterpret_cast<uintptr_t>(p.in) % in_vec || reinterpret_cast<uintptr_t>(p.out) % out_vec ||
+        reinterpret_cast<uintptr_t>(p.weight) % (4u * w))
+      return false;
+    for (int j = 0; j < 3; ++j)
+      if ((j == 2 ? p.heads : extent[j]) > 1 && (p.in_stride[j] * in_bytes % static_cast<int64_t>(in_vec) ||
+                                                 p.out_stride[j] * out_bytes % static_cast<int64_t>(out_vec)))
+        return false;
+  }
+  return true;
+}
+
+template <typename TI, typename TO, int W>
+cudaError_t launch_vectors(const RopeArgs &a, cudaStream_t st) {
+  int log_g = 0;
+  while ((2 * W << log_g) < a.dim) ++log_g;
+  int y = 0;
+  for (const RopePart &p : a.part) y += (p.heads + kHeads - 1) / kHeads;
+  unsigned threads = 256;  // fewer where a sequence has fewer tokens
+  while (threads > 32 && (threads >> 1 >> log_g) >= static_cast<unsigned>(a.seq)) threads >>= 1;
+  const unsigned tokens = threads >> log_g;
+  const dim3 grid((a.seq + tokens - 1) / tokens, y, a.batch);
+  return a.half ? op_launch(rope_vec_kernel<TI, TO, true, W>, grid, threads, 0, st, a, log_g)
+                : op_launch(rope_vec_kernel<TI, TO, false, W>, grid, threads, 0, st, a, log_g);
+}
+
 template <typename TI, typename TO>
 cudaError_t launch_rope(const RopeArgs &a, int sms, cudaStream_t st) {
   const long long rows = static_cast<long long>(a.batch) * a.seq * a.heads;
+  if (a.batch < 65536 && a.heads < 65536) {  // the grid's limits
+    if (vectors_fit(a, 4, sizeof(TI), sizeof(TO))) return launch_vectors<TI, TO, 4>(a, st);
+    if (vectors_fit(a, 2, sizeof(TI), sizeof(TO))) return launch_vectors<TI, TO, 2>(a, st);
+  }
   const long long blocks = (rows + kRopeWarps - 1) / kRopeWarps;
   const unsigned grid = static_cast<unsigned>(blocks < 32LL * sms ? blocks : 32LL * sms);
   return op_launch(rope_row_kernel<TI, TO>, dim3(grid), kRopeWarps * 32, 0, st, a);
@@ -210,6 +431,7 @@ extern "C" int htpg_qkv_rope(const struct htpg_rope_params *p, void *q_out, void
   a.half = p->layout == HTPG_ROPE_HALF;
   a.table_rows = p->table_rows;
   a.eps = p->eps;
+  a.inv_dim = 1.0f / static_cast<float>(p->head_dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p->in_type == HTPG_TYPE_F32) return op_result(launch_rope_out<float>(p->out_type, a, d.sms, st));
   if (p->in_type == HTPG_TYPE_F16) return op_result(launch_rope_out<__half>(p->out_type, a, d.sms, st));
