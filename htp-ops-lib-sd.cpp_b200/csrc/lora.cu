@@ -31,49 +31,79 @@ constexpr int kLoraThreads = 256, kLoraWarps = 8;
 // more products than (rows / BS + adapters in the tile) blocks.
 template <int TM>
 struct RowBlocks {
-  int row[TM];                            // row of the tile at each place of the order
+  int row[TM];                       // row of the tile at each place of the order
+  int rank[TM];                      // of its adapter; 0 without one
+  float scale[TM];
   int key[TM], ordered[TM], first[TM];
   int start[TM], count[TM], adapter[TM];  // per block; adapter -1: none
   int blocks;
 };
 
+constexpr int kNoAdapter = 0x7fffffff;
+
 template <int TM, int BS>
 __device__ void find_blocks(RowBlocks<TM> &r, const LoraArgs &p, int row0) {
   const int i = threadIdx.x, rows = min(TM, p.m - row0);
-  int key = 0;
+  int key = kNoAdapter, head = p.ids[row0];
+  if (head < 0 || head >= p.adapters) head = kNoAdapter;
   if (i < rows) {
     key = p.ids[row0 + i];
-    if (key < 0 || key >= p.adapters) key = 0x7fffffff;
+    if (key < 0 || key >= p.adapters) key = kNoAdapter;
     r.key[i] = key;
   }
-  __syncthreads();
-  if (i < rows) {
-    int place = 0;
-    for (int j = 0; j < rows; ++j) place += r.key[j] < key || (r.key[j] == key && j < i);
-    r.row[place] = i;
-    r.ordered[place] = key;
+  if (__syncthreads_and(i >= rows || key == head)) {  // one adapter
+    if (i < rows) {
+      r.row[i] = i;
+      const int block = i / BS;
+      if (i % BS == 0) {
+        r.start[block] = i;
+        r.count[block] = min(BS, rows - i);
+        r.adapter[block] = key == kNoAdapter ? -1 : key;
+      }
+    }
+    if (i == 0) r.blocks = (rows + BS - 1) / BS;
+  } else {
+    if (i < rows) {
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < rows; ++j) place += r.key[j] < key || (r.key[j] == key && j < i);
+      r.row[place] = i;
+      r.ordered[place] = key;
+    }
+    __syncthreads();
+    if (i < rows) {
+      int before = 0;
+      key = r.ordered[i];
+#pragma unroll 8
+      for (int j = 0; j < i; ++j) before += r.ordered[j] == key;
+      r.first[i] = before % BS == 0;
+    }
+    __syncthreads();
+    if (i < rows && r.first[i]) {
+      int block = 0, n = 1;
+#pragma unroll 8
+      for (int j = 0; j < i; ++j) block += r.first[j];
+      while (n < BS && i + n < rows && r.ordered[i + n] == key) ++n;
+      r.start[block] = i;
+      r.count[block] = n;
+      r.adapter[block] = key == kNoAdapter ? -1 : key;
+      if (i + n == rows) r.blocks = block + 1;
+    }
   }
-  __syncthreads();
-  int before = 0;
-  if (i < rows) {
-    key = r.ordered[i];
-    for (int j = 0; j < i; ++j) before += r.ordered[j] == key;
-    r.first[i] = before % BS == 0;
-  }
-  __syncthreads();
-  if (i < rows && r.first[i]) {
-    int block = 0, n = 1;
-    for (int j = 0; j < i; ++j) block += r.first[j];
-    while (n < BS && i + n < rows && r.ordered[i + n] == key) ++n;
-    r.start[block] = i;
-    r.count[block] = n;
-    r.adapter[block] = key == 0x7fffffff ? -1 : key;
-    if (i + n == rows) r.blocks = block + 1;
+  if (i < rows) {  // key: that of place i
+    r.rank[i] = key == kNoAdapter ? 0 : min(max(p.ranks[key], 0), p.max_rank);
+    r.scale[i] = key == kNoAdapter ? 0.0f : p.scales[key];
   }
   __syncthreads();
 }
 
-__device__ __forceinline__ int rank_of(const LoraArgs &p, int s) { return min(max(p.ranks[s], 0), p.max_rank); }
+// Waits, without regard to the CTA's abort flag but no longer than the limit,
+// for a bulk copy that is still landing.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < kWaitLimitNs) {
+  }
+}
 
 // ---------------------------------------------------------------- x A^T
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -83,121 +113,152 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Partial sums over K range blockIdx.y of t = x A^T for a tile's blocks
-// blockIdx.z, + gridDim.z, ...: part[range][row][max_rank].  The warps split
-// the range by 32-element steps; within a step lane t of a quad holds elements
-// 8t .. 8t + 7 of its rows of x and of A (any order of k will do, as long as
-// both sides have it), so every load is 16 or 32 contiguous bytes.
-// x = hi + lo, hi with the 11 significant bits that TF32 keeps, lo the rest,
-// which TF32 cuts to 11 more; A is exact in TF32.  The accumulators are added
-// up outside of the tensor core every kRun steps, whose own sums round towards zero.
-constexpr int kRun = 8;
+// Shared memory of the down kernel.  A stage holds kChunk elements of K of up
+// to 32 rows of x (FP32) and of the adapter's rows of A.  Row pitches are an odd
+// multiple of 64 bytes (x, read 16 bytes per lane) and 32 bytes past a multiple
+// of 128 (A, 8 bytes per lane), which spreads a fragment's rows over all banks.
+template <int RK>
+struct DownSmem {
+  static constexpr int kChunk = 128, kX = kChunk * 4 + 64, kA = kChunk * 2 + 32;
+  static constexpr int kStage = 32 * kX + RK * kA, kStages = RK >= 64 ? 2 : 3;
+  static constexpr int kRed = kStages * kStage;
+  static constexpr int kBytes = kRed + kLoraWarps * (RK / 8) * 32 * 16;
+};
 
-template <typename T, int RK, int MB>
-__global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_constant__ LoraArgs p, float *part,
-                                                                 int k_range) {
-  constexpr int TM = 32, NT = RK / 8;
+// Partial sums over K range blockIdx.y of t = x A^T for a tile's blocks
+// blockIdx.z, + gridDim.z, ...: part[range][row][max_rank].  Warp 8 brings the
+// blocks' rows in by bulk copies, one row piece each, running ahead over the
+// stages and into the next block; warps 0-7 split a stage's chunk of K (and the
+// rows, where there are more than 16).  Lane t of a quad holds elements 4t .. 4t +
+// 3 of each 16 of its rows of x and of A (any order of k will do, as long as
+// both sides have it).  x = hi + lo, hi with the 11 significant bits that TF32
+// keeps, lo the rest, which TF32 cuts to 11 more; A is exact in TF32.  The tensor
+// core's own sums round towards zero, so every stage's are added up outside of it (in shared memory).
+template <typename T, int RK>
+__global__ void __launch_bounds__(kLoraThreads + 32, RK == 128 ? 1 : 2)
+    lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range, uint32_t *watchdog) {
+  using S = DownSmem<RK>;
+  constexpr int TM = 32, NT = RK / 8, NS = S::kStages;
   __shared__ RowBlocks<TM> rb;
-  __shared__ float4 red[4][NT * MB][32];
+  __shared__ __align__(8) uint64_t bars[2 * NS];
+  __shared__ uint32_t abort_flag;
+  extern __shared__ __align__(128) uint8_t smem[];
+  volatile uint32_t *abort = &abort_flag;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * NS;
+  if (threadIdx.x == 0) {
+    *abort = 0;
+    for (int i = 0; i < NS; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, kLoraWarps);
+    fence_barrier_init();
+  }
   grid_dependency_wait();
   grid_dependents_launch();
   const int row0 = blockIdx.x * TM;
-  find_blocks<TM, 16 * MB>(rb, p, row0);
+  find_blocks<TM, 32>(rb, p, row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = blockIdx.y * k_range, k1 = min(k0 + k_range, p.k);
   part += static_cast<long long>(blockIdx.y) * p.m * p.max_rank;
+  uint32_t n = 0;  // stages so far
+  if (warp == kLoraWarps) {
+    bool ok = true;
+    for (int block = blockIdx.z; ok && block < rb.blocks; block += gridDim.z) {
+      const int start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
+      if (rank == 0) continue;
+      const T *a = static_cast<const T *>(p.a) + static_cast<long long>(rb.adapter[block]) * p.max_rank * p.k;
+      const float *x = lane < count ? p.x + (row0 + rb.row[start + lane]) * p.ldx : nullptr;
+      for (int k = k0; k < k1; k += S::kChunk, ++n) {
+        const uint32_t s = n % NS, bar = full + 8 * s, at = smem_u32(smem) + s * S::kStage;
+        const uint32_t kc = min(S::kChunk, k1 - k);
+        ok = mbar_wait(empty + 8 * s, (n / NS & 1u) ^ 1u, watchdog, kWatchProducer, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar, kc * 4 * count + kc * 2 * rank);
+        __syncwarp();
+        if (x) bulk_load(at + lane * S::kX, x + k, kc * 4, bar);
+        for (int r = lane; r < rank; r += 32)
+          bulk_load(at + 32 * S::kX + r * S::kA, a + static_cast<long long>(r) * p.k + k, kc * 2, bar);
+      }
+    }
+    // never leave the CTA with a copy still landing in its shared memory
+    for (uint32_t i = n > NS ? n - NS : 0; i < n; ++i) drain(full + 8 * (i % NS), i / NS & 1u);
+    return;
+  }
+  bool ok = true;
+  float4 *red = reinterpret_cast<float4 *>(smem + S::kRed);
   for (int block = blockIdx.z; block < rb.blocks; block += gridDim.z) {
-    const int s = rb.adapter[block];
-    if (s < 0) continue;
-    const int rank = rank_of(p, s), start = rb.start[block], count = rb.count[block];
-    const T *a = static_cast<const T *>(p.a) + static_cast<long long>(s) * p.max_rank * p.k;
-    const float *x[2 * MB];
+    const int start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
+    if (rank == 0) continue;
+    // 16 elements of K at a time: eight warps, or four for each half of the rows
+    const bool halves = count > 16;
+    const int half = halves ? warp & 1 : 0, first = (halves ? warp >> 1 : warp) * 16, step = halves ? 64 : 128;
+    float4 *sum = red + warp * NT * 32 + lane;  // this lane's
+    for (int k = k0; k < k1; k += S::kChunk, ++n) {
+      const uint32_t s = n % NS;
+      const int kc = min(S::kChunk, k1 - k);
+      ok = ok && mbar_wait(full + 8 * s, n / NS & 1u, watchdog, kWatchMma, abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      const uint8_t *xs = smem + s * S::kStage + (half * 16 + g) * S::kX, *as = smem + s * S::kStage + 32 * S::kX + g * S::kA;
+      float c[NT][4];
 #pragma unroll
-    for (int i = 0; i < 2 * MB; ++i)
-      x[i] = g + 8 * i < count ? p.x + (row0 + rb.row[start + g + 8 * i]) * p.ldx : nullptr;
-    float sum[MB][NT][4];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) sum[i][j][0] = sum[i][j][1] = sum[i][j][2] = sum[i][j][3] = 0.0f;
-    for (int kb = k0 + warp * 32; kb < k1; kb += kLoraWarps * 32) {
-      const int k = kb + 8 * t;
-      const bool in = k < k1;
-      float v[2 * MB][8];
-#pragma unroll
-      for (int i = 0; i < 2 * MB; ++i) {
-        float4 lo = make_float4(0, 0, 0, 0), hi = lo;
-        if (in && x[i]) {
-          lo = *reinterpret_cast<const float4 *>(x[i] + k);
-          hi = *reinterpret_cast<const float4 *>(x[i] + k + 4);
+      for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+      for (int q = first; q < kc; q += step) {
+        const int at = q + 4 * t;
+        const bool in = at < kc;  // the last 16 may hold 8
+        float4 v0 = make_float4(0, 0, 0, 0), v1 = v0;
+        uint2 w[NT];
+        if (in) {
+          v0 = *reinterpret_cast<const float4 *>(xs + at * 4);
+          v1 = *reinterpret_cast<const float4 *>(xs + 8 * S::kX + at * 4);
         }
-        v[i][0] = lo.x, v[i][1] = lo.y, v[i][2] = lo.z, v[i][3] = lo.w;
-        v[i][4] = hi.x, v[i][5] = hi.y, v[i][6] = hi.z, v[i][7] = hi.w;
-      }
-      uint4 w[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        w[j] = make_uint4(0, 0, 0, 0);
-        if (in && 8 * j + g < rank) w[j] = *reinterpret_cast<const uint4 *>(a + static_cast<long long>(8 * j + g) * p.k + k);
-      }
+        for (int j = 0; j < NT; ++j) w[j] = in ? *reinterpret_cast<const uint2 *>(as + 8 * j * S::kA + at * 2) : make_uint2(0, 0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t xh[MB][4], xl[MB][4];
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
+        for (int e = 0; e < 2; ++e) {
+          // a0, a1: rows g, g + 8 of element 2e; a2, a3: of element 2e + 1
+          const float f[4] = {e ? v0.z : v0.x, e ? v1.z : v1.x, e ? v0.w : v0.y, e ? v1.w : v1.y};
+          uint32_t xh[4], xl[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            // a0, a1: rows g, g + 8 of element 2e; a2, a3: of element 2e + 1
-            const float f = v[2 * i + (y & 1)][2 * e + (y >> 1)];
-            xh[i][y] = __float_as_uint(f) & 0xffffe000u;
-            xl[i][y] = __float_as_uint(f - __uint_as_float(xh[i][y]));
+            xh[y] = __float_as_uint(f[y]) & 0xffffe000u;
+            xl[y] = __float_as_uint(f[y] - __uint_as_float(xh[y]));
           }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float2 b = unpack2<T>(e == 0 ? w[j].x : e == 1 ? w[j].y : e == 2 ? w[j].z : w[j].w);
-          const uint32_t b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y);
+          for (int j = 0; j < NT; ++j) {
+            const float2 b = unpack2<T>(e ? w[j].y : w[j].x);
+            mma_tf32(c[j], xl, __float_as_uint(b.x), __float_as_uint(b.y));
+          }
 #pragma unroll
-          for (int i = 0; i < MB; ++i) {
-            mma_tf32(sum[i][j], xl[i], b0, b1);
-            mma_tf32(sum[i][j], xh[i], b0, b1);
+          for (int j = 0; j < NT; ++j) {
+            const float2 b = unpack2<T>(e ? w[j].y : w[j].x);
+            mma_tf32(c[j], xh, __float_as_uint(b.x), __float_as_uint(b.y));
           }
         }
       }
-    }
-    // the warps' sums, in a fixed tree
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + 8 * s);
 #pragma unroll
-    for (int half = kLoraWarps / 2; half > 0; half /= 2) {
-      __syncthreads();
-      if (warp >= half && warp < 2 * half) {
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            red[warp - half][i * NT + j][lane] = make_float4(sum[i][j][0], sum[i][j][1], sum[i][j][2], sum[i][j][3]);
-      }
-      __syncthreads();
-      if (warp < half) {
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const float4 o = red[warp][i * NT + j][lane];
-            sum[i][j][0] += o.x, sum[i][j][1] += o.y, sum[i][j][2] += o.z, sum[i][j][3] += o.w;
-          }
+      for (int j = 0; j < NT; ++j) {
+        const float4 o = k == k0 ? make_float4(0, 0, 0, 0) : sum[j * 32];
+        sum[j * 32] = make_float4(o.x + c[j][0], o.y + c[j][1], o.z + c[j][2], o.w + c[j][3]);
       }
     }
-    if (warp == 0) {
-#pragma unroll
-      for (int i = 0; i < 2 * MB; ++i) {
-        if (g + 8 * i >= count) continue;
-        float *out = part + static_cast<long long>(row0 + rb.row[start + g + 8 * i]) * p.max_rank;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (8 * j + 2 * t < p.max_rank)
-            *reinterpret_cast<float2 *>(out + 8 * j + 2 * t) =
-                make_float2(sum[i / 2][j][i % 2 * 2], sum[i / 2][j][i % 2 * 2 + 1]);
+    // the warps' sums, in order
+    named_bar_sync(1, kLoraThreads);
+    for (int i = threadIdx.x; i < (halves ? 2 : 1) * NT * 32; i += kLoraThreads) {
+      const int h = i / (NT * 32), j = i / 32 % NT, l = i % 32;
+      float4 o = make_float4(0, 0, 0, 0);
+      for (int w = h; w < kLoraWarps; w += halves ? 2 : 1) {
+        const float4 v = red[(w * NT + j) * 32 + l];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
       }
+      const int r = 8 * j + 2 * (l & 3), place = h * 16 + (l >> 2);
+      if (r >= p.max_rank || !ok) continue;
+      if (place < count)
+        *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place]) * p.max_rank + r) = make_float2(o.x, o.y);
+      if (place + 8 < count)
+        *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place + 8]) * p.max_rank + r) = make_float2(o.z, o.w);
     }
+    named_bar_sync(1, kLoraThreads);
   }
 }
 
@@ -216,178 +277,240 @@ __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A tile of rows x 256 columns, 32 columns per warp.  t (the sum of the ranges,
+template <typename T, int RK>
+struct UpSmem {
+  static constexpr int TM = RK == 128 ? 32 : 64, PITCH = RK + 8;
+  static constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+  static constexpr int kDepth = 3;      // blocks of base in flight per warp
+  static constexpr int kRow = 128 + 64;  // bytes from row to row: 16-byte reads of 8 rows spread over the banks
+  static constexpr int kBytes = kLoraWarps * kDepth * 16 * kRow;
+};
+
+// A tile of rows, its blocks blockIdx.z, + gridDim.z, ..., and the column range
+// blockIdx.y, 32 columns per warp at a time.  t (the sum of the K ranges,
 // times the adapter's scale) becomes the 16-bit A operand in parts that add up
 // to its FP32 value: two for FP16, the row scaled by a power of two to a
 // largest element in [2^10, 2^11) (undone at the end), so that what the parts
 // leave out is below 2^-22 of an element or 2^-35 of the row's largest; three for BF16.
 // Lane t of a quad holds ranks 4t .. 4t + 3 of each 16, and columns 4t .. 4t + 3
-// of each 16 in two MMA tiles, so that B, base and out move in 8- and 16-byte pieces.
+// of each 16 in two MMA tiles, so that B, base and out move in 8- and 16-byte
+// pieces.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
+// flight in a ring of its own, one bulk copy per row.
 template <typename T, int RK>
-__global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part,
-                                                               int ranges) {
-  constexpr int TM = RK == 128 ? 32 : 64, KS = RK / 16, PITCH = RK + 8;
-  constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+__global__ void __launch_bounds__(kLoraThreads, 2)
+    lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range, uint32_t *watchdog) {
+  using S = UpSmem<T, RK>;
+  constexpr int TM = S::TM, KS = RK / 16, PITCH = S::PITCH, PARTS = S::PARTS, D = S::kDepth;
   __shared__ RowBlocks<TM> rb;
-  __shared__ __align__(16) T ts[PARTS][TM][PITCH];  // by place in the order
   __shared__ float undo[TM];
+  __shared__ __align__(8) uint64_t bars[kLoraWarps * D];
+  __shared__ uint32_t abort_flag;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(16) T ts[PARTS][TM][PITCH];
+  volatile uint32_t *abort = &abort_flag;
+  if (threadIdx.x == 0) {
+    *abort = 0;
+    for (int i = 0; i < kLoraWarps * D; ++i) mbar_init(smem_u32(bars + i), 1);
+    fence_barrier_init();
+  }
   // what the kernel before the down pass wrote is visible: that pass waited for
   // it before it let this one start
   const int row0 = blockIdx.x * TM;
   find_blocks<TM, 16>(rb, p, row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int z = blockIdx.z, zs = gridDim.z;
+  const int mine = (rb.blocks - z + zs - 1) / zs;  // blocks of this CTA
+  const bool in_place = p.base == p.out && p.ldb == p.ldo;
+  // work: column groups of 32 (this warp's), each over the CTA's blocks
+  const int c_first = blockIdx.y * n_range + warp * 32, c_end = min(static_cast<int>(blockIdx.y + 1) * n_range, p.n);
+  const int groups = c_first < c_end ? (c_end - c_first + kLoraWarps * 32 - 1) / (kLoraWarps * 32) : 0;
+  const int items = groups * mine;
+  const uint8_t *ring = smem + warp * (D * 16 * S::kRow);
+  const uint32_t bar0 = smem_u32(bars + warp * D);
+  int f_group = 0, f_block = 0;  // of the next item to fetch
+  auto fetch = [&](int item) {
+    if (item >= items || !p.base) return;
+    const int block = z + f_block * zs, start = rb.start[block], count = rb.count[block];
+    const int c0 = c_first + f_group * (kLoraWarps * 32);
+    const uint32_t bytes = min(32, p.n - c0) * 4, bar = bar0 + 8 * (item % D);
+    __syncwarp();  // the slot's last reads
+    if (lane == 0) mbar_arrive_expect_tx(bar, bytes * count);
+    __syncwarp();
+    if (lane < count)
+      bulk_load(smem_u32(ring) + (item % D * 16 + lane) * S::kRow, p.base + (row0 + rb.row[start + lane]) * p.ldb + c0, bytes, bar);
+    if (++f_block == mine) f_block = 0, ++f_group;
+  };
   grid_dependency_wait();
-  for (int block = blockIdx.z; block < rb.blocks; block += gridDim.z) {
-    const int s = rb.adapter[block];
-    if (s < 0) continue;
-    const int rank = rank_of(p, s);
-    const float scale = p.scales[s];
-    for (int i = warp; i < 16; i += kLoraWarps) {
-      const int at = rb.start[block] + i;
-      if (i >= rb.count[block]) continue;
-      const float *src = part + static_cast<long long>(row0 + rb.row[at]) * p.max_rank;
-      float v[(RK + 31) / 32], most = 0.0f;
 #pragma unroll
-      for (int j = 0; j < (RK + 31) / 32; ++j) {
+  for (int i = 0; i < D - 1; ++i) fetch(i);
+  {
+    // one warp per place, every eighth, all of a warp's loads in flight together
+    constexpr int PLACES = TM / kLoraWarps, NV = (RK + 31) / 32;
+    const int rows = min(TM, p.m - row0);
+    float v[PLACES][NV];
+#pragma unroll
+    for (int u = 0; u < PLACES; ++u) {
+      const int at = warp + kLoraWarps * u;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
         const int r = lane + 32 * j;
-        v[j] = 0.0f;
-        if (r < rank)
-          for (int range = 0; range < ranges; ++range) v[j] += src[static_cast<long long>(range) * p.m * p.max_rank + r];
-        v[j] *= scale;
-        most = fmaxf(most, fabsf(v[j]));
+        v[u][j] = 0.0f;
+        if (at >= rows || r >= rb.rank[at]) continue;
+        const float *src = part + static_cast<long long>(row0 + rb.row[at]) * p.max_rank + r;
+        for (int range = 0; range < ranges; ++range) v[u][j] += src[static_cast<long long>(range) * p.m * p.max_rank];
+        v[u][j] *= rb.scale[at];
       }
+    }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int u = 0; u < PLACES; ++u) {
+      const int at = warp + kLoraWarps * u;
       float up = 1.0f, down = 1.0f;
-      if (PARTS == 2 && most > 0.0f && most < INFINITY) {
-        const int e = max(ilogbf(most), -110);
-        up = ldexpf(1.0f, 10 - e);
-        down = ldexpf(1.0f, e - 10);
+      if (PARTS == 2) {
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) most = fmaxf(most, fabsf(v[u][j]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // 2^(10 - e), e the exponent of the largest (subnormals: the nearest that stays finite)
+        if (most > 0.0f && most < INFINITY) {
+          const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -110);
+          up = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
+          down = __uint_as_float(static_cast<uint32_t>(127 + e - 10) << 23);
+        }
       }
       if (lane == 0) undo[at] = down;
 #pragma unroll
-      for (int j = 0; j < (RK + 31) / 32; ++j) {
+      for (int j = 0; j < NV; ++j) {
         const int r = lane + 32 * j;
         if (r >= RK) continue;
-        float rest = v[j] * up;
+        float rest = v[u][j] * up;
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
           const T h = from_f32<T>(rest);
           ts[q][at][r] = h;
-          rest = isfinite(rest) ? rest - to_f32(h) : 0.0f;
+          rest = fabsf(to_f32(h)) < INFINITY ? rest - to_f32(h) : 0.0f;
         }
       }
     }
   }
   __syncthreads();
-  const int c0 = blockIdx.y * (kLoraWarps * 32) + warp * 32;
-  if (c0 >= p.n) return;
-  const bool in_place = p.base == p.out && p.ldb == p.ldo;
   uint2 w[4][KS];
-  int held = -1;
-  for (int block = blockIdx.z; block < rb.blocks; block += gridDim.z) {
-    const int s = rb.adapter[block], start = rb.start[block], count = rb.count[block];
-    const int rank = s < 0 ? 0 : rank_of(p, s);
-    if (rank == 0 && in_place) continue;
-    float4 o[2][2];
-    long long row[2];
+  int held = -1, held_group = -1, group = 0, at = 0;
+  for (int item = 0; item < items; ++item) {
+    fetch(item + D - 1);
+    const int block = z + at * zs, c0 = c_first + group * (kLoraWarps * 32);
+    const int s = rb.adapter[block], start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
+    if (rank && (s != held || group != held_group)) {
+      held = s, held_group = group;
+      const T *b = static_cast<const T *>(p.b) + static_cast<long long>(s) * p.n * p.max_rank;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool ok = g + 8 * i < count;
-      row[i] = ok ? row0 + rb.row[start + g + 8 * i] : -1;
+      for (int j = 0; j < 4; ++j) {
+        const int c = c0 + 16 * (j >> 1) + 4 * (g >> 1) + 2 * (j & 1) + (g & 1);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = c0 + 16 * h + 4 * t;
-        o[i][h] = make_float4(0, 0, 0, 0);
-        if (ok && p.base && c < p.n) o[i][h] = __ldcs(reinterpret_cast<const float4 *>(p.base + row[i] * p.ldb + c));
-      }
-    }
-    if (rank) {
-      if (s != held) {
-        held = s;
-        const T *b = static_cast<const T *>(p.b) + static_cast<long long>(s) * p.n * p.max_rank;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = c0 + 16 * (j >> 1) + 4 * (g >> 1) + 2 * (j & 1) + (g & 1);
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const int r = 16 * k + 4 * t;
-            w[j][k] = make_uint2(0, 0);
-            if (c < p.n && r < rank) {
-              w[j][k] = *reinterpret_cast<const uint2 *>(b + static_cast<long long>(c) * p.max_rank + r);
-              if (r + 1 >= rank) w[j][k].x &= 0xffffu;
-              if (r + 2 >= rank) w[j][k].y = 0;
-              if (r + 3 >= rank) w[j][k].y &= 0xffffu;
-            }
-          }
+        for (int k = 0; k < KS; ++k) {
+          const int r = 16 * k + 4 * t;
+          w[j][k] = make_uint2(0, 0);
+          if (c < p.n && r < rank) w[j][k] = *reinterpret_cast<const uint2 *>(b + static_cast<long long>(c) * p.max_rank + r);
         }
       }
+      if (rank % 4) {  // what lies past the rank may be anything
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            const int left = rank - (16 * k + 4 * t);
+            if (left < 4) w[j][k].y &= left == 3 ? 0xffffu : 0u;
+            if (left < 2) w[j][k].x &= left == 1 ? 0xffffu : 0u;
+          }
+      }
+    }
+    if (++at == mine) at = 0, ++group;
+    if (p.base) {
+      const bool ok = mbar_wait(bar0 + 8 * (item % D), item / D & 1u, watchdog, kWatchEpilogue, abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        for (int i = item; i < min(item + D, items); ++i) drain(bar0 + 8 * (i % D), i / D & 1u);
+        break;
+      }
+    }
+    if (rank == 0 && in_place) continue;
+    float4 o[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o[i][h] = p.base ? *reinterpret_cast<const float4 *>(ring + (item % D * 16 + g + 8 * i) * S::kRow + h * 64 + t * 16)
+                         : make_float4(0, 0, 0, 0);
+    if (rank) {
       float acc[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+      // places past the block's rows: those of other blocks, whose results are not stored
+      const int r0 = min(start + g, TM - 1), r1 = min(start + g + 8, TM - 1);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         if (16 * k >= rank) break;
 #pragma unroll
         for (int q = PARTS - 1; q >= 0; --q) {
-          uint32_t a[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (row[i] < 0) continue;
-            const uint2 v = *reinterpret_cast<const uint2 *>(&ts[q][start + g + 8 * i][16 * k + 4 * t]);
-            a[i] = v.x, a[2 + i] = v.y;
-          }
+          const uint2 v0 = *reinterpret_cast<const uint2 *>(&ts[q][r0][16 * k + 4 * t]);
+          const uint2 v1 = *reinterpret_cast<const uint2 *>(&ts[q][r1][16 * k + 4 * t]);
+          const uint32_t a[4] = {v0.x, v1.x, v0.y, v1.y};
 #pragma unroll
           for (int j = 0; j < 4; ++j) mma_16<T>(acc[j], a, w[j][k].x, w[j][k].y);
         }
       }
+      const float down[2] = {undo[r0], undo[r1]};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (row[i] < 0) continue;
-        const float down = undo[start + g + 8 * i];
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          o[i][h].x = fmaf(acc[2 * h][2 * i], down, o[i][h].x);
-          o[i][h].y = fmaf(acc[2 * h][2 * i + 1], down, o[i][h].y);
-          o[i][h].z = fmaf(acc[2 * h + 1][2 * i], down, o[i][h].z);
-          o[i][h].w = fmaf(acc[2 * h + 1][2 * i + 1], down, o[i][h].w);
+          o[i][h].x = fmaf(acc[2 * h][2 * i], down[i], o[i][h].x);
+          o[i][h].y = fmaf(acc[2 * h][2 * i + 1], down[i], o[i][h].y);
+          o[i][h].z = fmaf(acc[2 * h + 1][2 * i], down[i], o[i][h].z);
+          o[i][h].w = fmaf(acc[2 * h + 1][2 * i + 1], down[i], o[i][h].w);
         }
-      }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      if (g + 8 * i >= count) continue;
+      float *out = p.out + (row0 + rb.row[start + g + 8 * i]) * p.ldo;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c = c0 + 16 * h + 4 * t;
-        if (row[i] >= 0 && c < p.n) __stcs(reinterpret_cast<float4 *>(p.out + row[i] * p.ldo + c), o[i][h]);
+        if (c < p.n) __stcs(reinterpret_cast<float4 *>(out + c), o[i][h]);
       }
+    }
   }
 }
 
 template <typename T, int RK>
 int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
-  // Down: ranges of K until the SMs have a block each (no shorter than one step
-  // per warp), and blocks of few tiles side by side.
-  constexpr int MB = RK == 128 ? 1 : 2;
+  // Down: ranges of K until the SMs have a block each (no shorter than two
+  // stages), and blocks of few tiles side by side.
+  using D = DownSmem<RK>;
   const int tiles = (p.m + 31) / 32;
-  const int steps = (p.k + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
+  const int steps = (p.k + 2 * D::kChunk - 1) / (2 * D::kChunk);
   const int ranges = std::max(1, std::min(steps, d.sms / tiles));
-  const int k_range = (steps + ranges - 1) / ranges * kLoraWarps * 32;
-  const int z_down = std::max(1, std::min({8, p.adapters, p.m, 2 * d.sms / (tiles * ranges)}));
-  constexpr int TM = RK == 128 ? 32 : 64;
-  const int up_tiles = (p.m + TM - 1) / TM, n_tiles = (p.n + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
-  const int z_up = std::max(1, std::min({8, p.adapters, p.m, 4 * d.sms / (up_tiles * n_tiles)}));
+  const int k_range = (steps + ranges - 1) / ranges * 2 * D::kChunk;
+  const int k_ranges = (p.k + k_range - 1) / k_range;
+  const int z_down = std::max(1, std::min({8, p.adapters, p.m, d.sms / (tiles * k_ranges)}));
+  // Up: column ranges until every SM has two blocks, then blocks of rows side by side.
+  using U = UpSmem<T, RK>;
+  const int up_tiles = (p.m + U::TM - 1) / U::TM, n_steps = (p.n + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
+  const int want = std::max(1, std::min(n_steps, 2 * d.sms / up_tiles));
+  const int n_range = (n_steps + want - 1) / want * kLoraWarps * 32, n_ranges = (p.n + n_range - 1) / n_range;
+  const int z_up = std::max(1, std::min({8, p.adapters, p.m, 2 * d.sms / (up_tiles * n_ranges)}));
   auto lock = op_lock();
   uint32_t *counters;
   uint8_t *scratch;
-  const int rc = op_scratch(st, static_cast<size_t>(ranges) * p.m * p.max_rank * sizeof(float), &counters, &scratch);
+  const int rc = op_scratch(st, static_cast<size_t>(k_ranges) * p.m * p.max_rank * sizeof(float), &counters, &scratch);
   if (rc) return rc;
   float *part = reinterpret_cast<float *>(scratch);
-  cudaError_t e = op_launch(lora_down_kernel<T, RK, MB>, dim3(tiles, (p.k + k_range - 1) / k_range, z_down), kLoraThreads,
-                            0, st, p, part, k_range);
-  if (e == cudaSuccess)
-    e = op_launch(lora_up_kernel<T, RK>, dim3(up_tiles, n_tiles, z_up), kLoraThreads, 0, st, p, part,
-                  (p.k + k_range - 1) / k_range);
+  auto *down = lora_down_kernel<T, RK>;
+  auto *up = lora_up_kernel<T, RK>;
+  cudaError_t e = cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, D::kBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, U::kBytes);
+  if (e == cudaSuccess) e = op_launch(down, dim3(tiles, k_ranges, z_down), kLoraThreads + 32, D::kBytes, st, p, part, k_range, d.watchdog);
+  if (e == cudaSuccess) e = op_launch(up, dim3(up_tiles, n_ranges, z_up), kLoraThreads, U::kBytes, st, p, part, k_ranges, n_range, d.watchdog);
   return op_result(e);
 }
 
