@@ -97,12 +97,14 @@ __device__ void find_blocks(RowBlocks<TM> &r, const LoraArgs &p, int row0) {
   __syncthreads();
 }
 
-// Waits, without regard to the CTA's abort flag but no longer than the limit,
-// for a bulk copy that is still landing.
-__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer();
-  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < kWaitLimitNs) {
-  }
+// 16 bytes to shared memory, zeros where `in` is false (src is not read then).
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // ---------------------------------------------------------------- x A^T
@@ -113,43 +115,33 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Shared memory of the down kernel.  A stage holds kChunk elements of K of up
-// to 32 rows of x (FP32) and of the adapter's rows of A.  Row pitches are an odd
-// multiple of 64 bytes (x, read 16 bytes per lane) and 32 bytes past a multiple
-// of 128 (A, 8 bytes per lane), which spreads a fragment's rows over all banks.
+// Shared memory of the down kernel: a ring of steps per warp, a step's 16-byte
+// pieces by lane (every lane reads only what it copied: no barrier).
 template <int RK>
 struct DownSmem {
-  static constexpr int kChunk = 128, kX = kChunk * 4 + 64, kA = kChunk * 2 + 32;
-  static constexpr int kStage = 32 * kX + RK * kA, kStages = RK >= 64 ? 2 : 3;
-  static constexpr int kRed = kStages * kStage;
-  static constexpr int kBytes = kRed + kLoraWarps * (RK / 8) * 32 * 16;
+  static constexpr int kPieces = 4 + RK / 8;  // of two rows of x, of A
+  static constexpr int kSteps = RK == 128 ? 2 : 3;
+  static constexpr int kRing = kLoraWarps * kSteps * kPieces * 32 * 16;
+  static constexpr int kRed = kLoraWarps * (RK / 8) * 32 * 16;
+  static constexpr int kBytes = kRing > kRed ? kRing : kRed;
 };
 
 // Partial sums over K range blockIdx.y of t = x A^T for a tile's blocks
-// blockIdx.z, + gridDim.z, ...: part[range][row][max_rank].  Warp 8 brings the
-// blocks' rows in by bulk copies, one row piece each, running ahead over the
-// stages and into the next block; warps 0-7 split a stage's chunk of K (and the
-// rows, where there are more than 16).  Lane t of a quad holds elements 4t .. 4t +
-// 3 of each 16 of its rows of x and of A (any order of k will do, as long as
-// both sides have it).  x = hi + lo, hi with the 11 significant bits that TF32
-// keeps, lo the rest, which TF32 cuts to 11 more; A is exact in TF32.  The tensor
-// core's own sums round towards zero, so every stage's are added up outside of it (in shared memory).
+// blockIdx.z, + gridDim.z, ...: part[range][row][max_rank].  A warp has 16 rows
+// and every fourth or eighth 32-element step of the range (four warps for each
+// half of a block with more than 16 rows); within a step lane t of a quad holds
+// elements 8t .. 8t + 7 of its rows of x and of A (any order of k will do, as
+// long as both sides have it).  x = hi + lo, hi with the 11 significant bits
+// that TF32 keeps, lo the rest, which TF32 cuts to 11 more; A is exact in TF32.
+// The tensor core's own sums round towards zero, so they are added up outside
+// of it every step.
 template <typename T, int RK>
-__global__ void __launch_bounds__(kLoraThreads + 32, RK == 128 ? 1 : 2)
-    lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range, uint32_t *watchdog) {
+__global__ void __launch_bounds__(kLoraThreads, RK >= 64 ? 1 : 2)
+    lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range) {
   using S = DownSmem<RK>;
-  constexpr int TM = 32, NT = RK / 8, NS = S::kStages;
+  constexpr int TM = 32, NT = RK / 8, NS = S::kSteps;
   __shared__ RowBlocks<TM> rb;
-  __shared__ __align__(8) uint64_t bars[2 * NS];
-  __shared__ uint32_t abort_flag;
-  extern __shared__ __align__(128) uint8_t smem[];
-  volatile uint32_t *abort = &abort_flag;
-  const uint32_t full = smem_u32(bars), empty = full + 8 * NS;
-  if (threadIdx.x == 0) {
-    *abort = 0;
-    for (int i = 0; i < NS; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, kLoraWarps);
-    fence_barrier_init();
-  }
+  extern __shared__ __align__(16) uint4 smem[];
   grid_dependency_wait();
   grid_dependents_launch();
   const int row0 = blockIdx.x * TM;
@@ -157,93 +149,85 @@ __global__ void __launch_bounds__(kLoraThreads + 32, RK == 128 ? 1 : 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = blockIdx.y * k_range, k1 = min(k0 + k_range, p.k);
   part += static_cast<long long>(blockIdx.y) * p.m * p.max_rank;
-  uint32_t n = 0;  // stages so far
-  if (warp == kLoraWarps) {
-    bool ok = true;
-    for (int block = blockIdx.z; ok && block < rb.blocks; block += gridDim.z) {
-      const int start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
-      if (rank == 0) continue;
-      const T *a = static_cast<const T *>(p.a) + static_cast<long long>(rb.adapter[block]) * p.max_rank * p.k;
-      const float *x = lane < count ? p.x + (row0 + rb.row[start + lane]) * p.ldx : nullptr;
-      for (int k = k0; k < k1; k += S::kChunk, ++n) {
-        const uint32_t s = n % NS, bar = full + 8 * s, at = smem_u32(smem) + s * S::kStage;
-        const uint32_t kc = min(S::kChunk, k1 - k);
-        ok = mbar_wait(empty + 8 * s, (n / NS & 1u) ^ 1u, watchdog, kWatchProducer, abort);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(bar, kc * 4 * count + kc * 2 * rank);
-        __syncwarp();
-        if (x) bulk_load(at + lane * S::kX, x + k, kc * 4, bar);
-        for (int r = lane; r < rank; r += 32)
-          bulk_load(at + 32 * S::kX + r * S::kA, a + static_cast<long long>(r) * p.k + k, kc * 2, bar);
-      }
-    }
-    // never leave the CTA with a copy still landing in its shared memory
-    for (uint32_t i = n > NS ? n - NS : 0; i < n; ++i) drain(full + 8 * (i % NS), i / NS & 1u);
-    return;
-  }
-  bool ok = true;
-  float4 *red = reinterpret_cast<float4 *>(smem + S::kRed);
+  uint4 *ring = smem + warp * (NS * S::kPieces * 32) + lane;
+  float4 *red = reinterpret_cast<float4 *>(smem);
   for (int block = blockIdx.z; block < rb.blocks; block += gridDim.z) {
     const int start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
     if (rank == 0) continue;
-    // 16 elements of K at a time: eight warps, or four for each half of the rows
     const bool halves = count > 16;
-    const int half = halves ? warp & 1 : 0, first = (halves ? warp >> 1 : warp) * 16, step = halves ? 64 : 128;
-    float4 *sum = red + warp * NT * 32 + lane;  // this lane's
-    for (int k = k0; k < k1; k += S::kChunk, ++n) {
-      const uint32_t s = n % NS;
-      const int kc = min(S::kChunk, k1 - k);
-      ok = ok && mbar_wait(full + 8 * s, n / NS & 1u, watchdog, kWatchMma, abort);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) continue;
-      const uint8_t *xs = smem + s * S::kStage + (half * 16 + g) * S::kX, *as = smem + s * S::kStage + 32 * S::kX + g * S::kA;
+    const int row_a = (halves ? (warp & 1) * 16 : 0) + g, row_b = row_a + 8;  // of the block
+    const T *a = static_cast<const T *>(p.a) + static_cast<long long>(rb.adapter[block]) * p.max_rank * p.k +
+                 static_cast<long long>(g) * p.k;
+    const float *xa = p.x + (row0 + rb.row[start + min(row_a, count - 1)]) * p.ldx;
+    const float *xb = p.x + (row0 + rb.row[start + min(row_b, count - 1)]) * p.ldx;
+    const int k_first = k0 + (halves ? warp >> 1 : warp) * 32 + 8 * t, k_step = halves ? 128 : 256;
+    const long long a_step = 8LL * p.k;
+    auto load = [&](int k, int slot) {
+      const bool in = k < k1;
+      uint4 *to = ring + slot * (S::kPieces * 32);
+      copy16(to, xa + (in ? k : 0), in);
+      copy16(to + 32, xa + (in ? k + 4 : 0), in);
+      copy16(to + 64, xb + (in ? k : 0), in);
+      copy16(to + 96, xb + (in ? k + 4 : 0), in);
+      const T *from = a + (in ? k : 0);
+#pragma unroll
+      for (int j = 0; j < NT; ++j, from += a_step) {
+        const bool rank_in = in && 8 * j + g < rank;
+        copy16(to + (4 + j) * 32, rank_in ? from : a, rank_in);
+      }
+      copy_commit();
+    };
+    float sum[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) load(k_first + i * k_step, i);
+    int slot = 0;
+    for (int k = k_first; k - 8 * t < k1; k += k_step) {
+      load(k + (NS - 1) * k_step, slot == 0 ? NS - 1 : slot - 1);
+      copy_wait<NS - 1>();
+      const uint4 *from = ring + slot * (S::kPieces * 32);
+      slot = slot + 1 == NS ? 0 : slot + 1;
       float c[NT][4];
 #pragma unroll
       for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-      for (int q = first; q < kc; q += step) {
-        const int at = q + 4 * t;
-        const bool in = at < kc;  // the last 16 may hold 8
-        float4 v0 = make_float4(0, 0, 0, 0), v1 = v0;
-        uint2 w[NT];
-        if (in) {
-          v0 = *reinterpret_cast<const float4 *>(xs + at * 4);
-          v1 = *reinterpret_cast<const float4 *>(xs + 8 * S::kX + at * 4);
-        }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = in ? *reinterpret_cast<const uint2 *>(as + 8 * j * S::kA + at * 2) : make_uint2(0, 0);
+      for (int h = 0; h < 2; ++h) {  // elements 4h .. 4h + 3 of the lane's eight
+        const float4 va = *reinterpret_cast<const float4 *>(from + h * 32), vb = *reinterpret_cast<const float4 *>(from + (2 + h) * 32);
+        uint2 w[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[j] = reinterpret_cast<const uint2 *>(from + (4 + j) * 32)[h];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           // a0, a1: rows g, g + 8 of element 2e; a2, a3: of element 2e + 1
-          const float f[4] = {e ? v0.z : v0.x, e ? v1.z : v1.x, e ? v0.w : v0.y, e ? v1.w : v1.y};
+          const float f[4] = {e ? va.z : va.x, e ? vb.z : vb.x, e ? va.w : va.y, e ? vb.w : vb.y};
           uint32_t xh[4], xl[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             xh[y] = __float_as_uint(f[y]) & 0xffffe000u;
             xl[y] = __float_as_uint(f[y] - __uint_as_float(xh[y]));
           }
+          float2 b[NT];
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const float2 b = unpack2<T>(e ? w[j].y : w[j].x);
-            mma_tf32(c[j], xl, __float_as_uint(b.x), __float_as_uint(b.y));
+            b[j] = unpack2<T>(e ? w[j].y : w[j].x);
+            mma_tf32(c[j], xl, __float_as_uint(b[j].x), __float_as_uint(b[j].y));
           }
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const float2 b = unpack2<T>(e ? w[j].y : w[j].x);
-            mma_tf32(c[j], xh, __float_as_uint(b.x), __float_as_uint(b.y));
-          }
+          for (int j = 0; j < NT; ++j) mma_tf32(c[j], xh, __float_as_uint(b[j].x), __float_as_uint(b[j].y));
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + 8 * s);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const float4 o = k == k0 ? make_float4(0, 0, 0, 0) : sum[j * 32];
-        sum[j * 32] = make_float4(o.x + c[j][0], o.y + c[j][1], o.z + c[j][2], o.w + c[j][3]);
-      }
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) sum[j][y] += c[j][y];
     }
-    // the warps' sums, in order
-    named_bar_sync(1, kLoraThreads);
+    copy_wait<0>();
+    __syncthreads();  // the rings become the warps' sums, added in order
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      red[(warp * NT + j) * 32 + lane] = make_float4(sum[j][0], sum[j][1], sum[j][2], sum[j][3]);
+    __syncthreads();
     for (int i = threadIdx.x; i < (halves ? 2 : 1) * NT * 32; i += kLoraThreads) {
       const int h = i / (NT * 32), j = i / 32 % NT, l = i % 32;
       float4 o = make_float4(0, 0, 0, 0);
@@ -252,13 +236,13 @@ __global__ void __launch_bounds__(kLoraThreads + 32, RK == 128 ? 1 : 2)
         o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
       }
       const int r = 8 * j + 2 * (l & 3), place = h * 16 + (l >> 2);
-      if (r >= p.max_rank || !ok) continue;
+      if (r >= p.max_rank) continue;
       if (place < count)
         *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place]) * p.max_rank + r) = make_float2(o.x, o.y);
       if (place + 8 < count)
         *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place + 8]) * p.max_rank + r) = make_float2(o.z, o.w);
     }
-    named_bar_sync(1, kLoraThreads);
+    __syncthreads();
   }
 }
 
@@ -281,9 +265,8 @@ template <typename T, int RK>
 struct UpSmem {
   static constexpr int TM = RK == 128 ? 32 : 64, PITCH = RK + 8;
   static constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
-  static constexpr int kDepth = 3;      // blocks of base in flight per warp
-  static constexpr int kRow = 128 + 64;  // bytes from row to row: 16-byte reads of 8 rows spread over the banks
-  static constexpr int kBytes = kLoraWarps * kDepth * 16 * kRow;
+  static constexpr int kDepth = 4;  // blocks of base in flight per warp
+  static constexpr int kBytes = kLoraWarps * kDepth * 4 * 32 * 16;
 };
 
 // A tile of rows, its blocks blockIdx.z, + gridDim.z, ..., and the column range
@@ -295,24 +278,16 @@ struct UpSmem {
 // Lane t of a quad holds ranks 4t .. 4t + 3 of each 16, and columns 4t .. 4t + 3
 // of each 16 in two MMA tiles, so that B, base and out move in 8- and 16-byte
 // pieces.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
-// flight in a ring of its own, one bulk copy per row.
+// flight in a ring of its own, read back by the lanes that copied them.
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, 2)
-    lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range, uint32_t *watchdog) {
+    lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range) {
   using S = UpSmem<T, RK>;
   constexpr int TM = S::TM, KS = RK / 16, PITCH = S::PITCH, PARTS = S::PARTS, D = S::kDepth;
   __shared__ RowBlocks<TM> rb;
   __shared__ float undo[TM];
-  __shared__ __align__(8) uint64_t bars[kLoraWarps * D];
-  __shared__ uint32_t abort_flag;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(16) uint4 smem[];
   __shared__ __align__(16) T ts[PARTS][TM][PITCH];
-  volatile uint32_t *abort = &abort_flag;
-  if (threadIdx.x == 0) {
-    *abort = 0;
-    for (int i = 0; i < kLoraWarps * D; ++i) mbar_init(smem_u32(bars + i), 1);
-    fence_barrier_init();
-  }
   // what the kernel before the down pass wrote is visible: that pass waited for
   // it before it let this one start
   const int row0 = blockIdx.x * TM;
@@ -325,20 +300,23 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   const int c_first = blockIdx.y * n_range + warp * 32, c_end = min(static_cast<int>(blockIdx.y + 1) * n_range, p.n);
   const int groups = c_first < c_end ? (c_end - c_first + kLoraWarps * 32 - 1) / (kLoraWarps * 32) : 0;
   const int items = groups * mine;
-  const uint8_t *ring = smem + warp * (D * 16 * S::kRow);
-  const uint32_t bar0 = smem_u32(bars + warp * D);
+  uint4 *ring = smem + warp * (D * 4 * 32) + lane;
   int f_group = 0, f_block = 0;  // of the next item to fetch
   auto fetch = [&](int item) {
-    if (item >= items || !p.base) return;
-    const int block = z + f_block * zs, start = rb.start[block], count = rb.count[block];
-    const int c0 = c_first + f_group * (kLoraWarps * 32);
-    const uint32_t bytes = min(32, p.n - c0) * 4, bar = bar0 + 8 * (item % D);
-    __syncwarp();  // the slot's last reads
-    if (lane == 0) mbar_arrive_expect_tx(bar, bytes * count);
-    __syncwarp();
-    if (lane < count)
-      bulk_load(smem_u32(ring) + (item % D * 16 + lane) * S::kRow, p.base + (row0 + rb.row[start + lane]) * p.ldb + c0, bytes, bar);
-    if (++f_block == mine) f_block = 0, ++f_group;
+    if (item < items && p.base) {
+      const int block = z + f_block * zs, start = rb.start[block], count = rb.count[block];
+      const int c = c_first + f_group * (kLoraWarps * 32) + 4 * t;
+      uint4 *to = ring + item % D * (4 * 32);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float *src = p.base + (row0 + rb.row[start + min(g + 8 * i, count - 1)]) * p.ldb;
+        const bool ok = g + 8 * i < count;
+        copy16(to + 2 * i * 32, src + (c < p.n ? c : 0), ok && c < p.n);
+        copy16(to + (2 * i + 1) * 32, src + (c + 16 < p.n ? c + 16 : 0), ok && c + 16 < p.n);
+      }
+      if (++f_block == mine) f_block = 0, ++f_group;
+    }
+    copy_commit();
   };
   grid_dependency_wait();
 #pragma unroll
@@ -425,21 +403,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       }
     }
     if (++at == mine) at = 0, ++group;
-    if (p.base) {
-      const bool ok = mbar_wait(bar0 + 8 * (item % D), item / D & 1u, watchdog, kWatchEpilogue, abort);
-      if (!__all_sync(0xffffffffu, ok)) {
-        for (int i = item; i < min(item + D, items); ++i) drain(bar0 + 8 * (i % D), i / D & 1u);
-        break;
-      }
-    }
+    copy_wait<D - 1>();
     if (rank == 0 && in_place) continue;
     float4 o[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        o[i][h] = p.base ? *reinterpret_cast<const float4 *>(ring + (item % D * 16 + g + 8 * i) * S::kRow + h * 64 + t * 16)
-                         : make_float4(0, 0, 0, 0);
+        o[i][h] = p.base ? *reinterpret_cast<const float4 *>(ring + (item % D * 4 + 2 * i + h) * 32) : make_float4(0, 0, 0, 0);
     if (rank) {
       float acc[4][4];
 #pragma unroll
@@ -480,24 +451,32 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       }
     }
   }
+  copy_wait<0>();
 }
 
 template <typename T, int RK>
 int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
-  // Down: ranges of K until the SMs have a block each (no shorter than two
-  // stages), and blocks of few tiles side by side.
+  // Down: ranges of K until every SM has a block (none shorter than a step per
+  // warp), then blocks of one tile side by side.
+  using U = UpSmem<T, RK>;
   using D = DownSmem<RK>;
-  const int tiles = (p.m + 31) / 32;
-  const int steps = (p.k + 2 * D::kChunk - 1) / (2 * D::kChunk);
+  const int tiles = (p.m + 31) / 32, steps = (p.k + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
   const int ranges = std::max(1, std::min(steps, d.sms / tiles));
-  const int k_range = (steps + ranges - 1) / ranges * 2 * D::kChunk;
+  const int k_range = (steps + ranges - 1) / ranges * kLoraWarps * 32;
   const int k_ranges = (p.k + k_range - 1) / k_range;
   const int z_down = std::max(1, std::min({8, p.adapters, p.m, d.sms / (tiles * k_ranges)}));
-  // Up: column ranges until every SM has two blocks, then blocks of rows side by side.
-  using U = UpSmem<T, RK>;
+  // Up: the column ranges whose rounds of CTAs (two per SM) do least, a CTA's
+  // set-up counted as two steps of 256 columns; then blocks of rows side by side.
   const int up_tiles = (p.m + U::TM - 1) / U::TM, n_steps = (p.n + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
-  const int want = std::max(1, std::min(n_steps, 2 * d.sms / up_tiles));
-  const int n_range = (n_steps + want - 1) / want * kLoraWarps * 32, n_ranges = (p.n + n_range - 1) / n_range;
+  int n_range = n_steps;
+  long long least = -1;
+  for (int per = 1; per <= n_steps; ++per) {
+    const long long ctas = static_cast<long long>(up_tiles) * ((n_steps + per - 1) / per);
+    const long long cost = (ctas + 2 * d.sms - 1) / (2 * d.sms) * (per + 2);
+    if (least < 0 || cost <= least) least = cost, n_range = per;
+  }
+  n_range *= kLoraWarps * 32;
+  const int n_ranges = (p.n + n_range - 1) / n_range;
   const int z_up = std::max(1, std::min({8, p.adapters, p.m, 2 * d.sms / (up_tiles * n_ranges)}));
   auto lock = op_lock();
   uint32_t *counters;
@@ -509,8 +488,8 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   auto *up = lora_up_kernel<T, RK>;
   cudaError_t e = cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, D::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, U::kBytes);
-  if (e == cudaSuccess) e = op_launch(down, dim3(tiles, k_ranges, z_down), kLoraThreads + 32, D::kBytes, st, p, part, k_range, d.watchdog);
-  if (e == cudaSuccess) e = op_launch(up, dim3(up_tiles, n_ranges, z_up), kLoraThreads, U::kBytes, st, p, part, k_ranges, n_range, d.watchdog);
+  if (e == cudaSuccess) e = op_launch(down, dim3(tiles, k_ranges, z_down), kLoraThreads, D::kBytes, st, p, part, k_range);
+  if (e == cudaSuccess) e = op_launch(up, dim3(up_tiles, n_ranges, z_up), kLoraThreads, U::kBytes, st, p, part, k_ranges, n_range);
   return op_result(e);
 }
 
