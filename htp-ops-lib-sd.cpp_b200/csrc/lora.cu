@@ -261,9 +261,19 @@ __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Word i of a vector of words (i known when compiling).
+__device__ __forceinline__ uint32_t &word(uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t &word(uint2 &v, int i) { return i == 0 ? v.x : v.y; }
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint2 &v, int i) { return i == 0 ? v.x : v.y; }
+
 template <typename T, int RK>
 struct UpSmem {
-  static constexpr int TM = RK == 128 ? 32 : 64, PITCH = RK + 8;
+  static constexpr int TM = RK == 128 ? 32 : 64;
+  // elements from row to row: the rows of one access phase (2 of 64 bytes, 4 of
+  // 32 at rank 16) lie on different banks
+  static constexpr int PITCH = RK == 64 ? 96 : RK == 128 ? 160 : RK;
+  static constexpr int kVec = RK >= 32 ? 8 : 4;  // ranks a lane holds together
   static constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
   static constexpr int kDepth = 4;  // blocks of base in flight per warp
   static constexpr int kBytes = kLoraWarps * kDepth * 4 * 32 * 16;
@@ -275,15 +285,15 @@ struct UpSmem {
 // to its FP32 value: two for FP16, the row scaled by a power of two to a
 // largest element in [2^10, 2^11) (undone at the end), so that what the parts
 // leave out is below 2^-22 of an element or 2^-35 of the row's largest; three for BF16.
-// Lane t of a quad holds ranks 4t .. 4t + 3 of each 16, and columns 4t .. 4t + 3
-// of each 16 in two MMA tiles, so that B, base and out move in 8- and 16-byte
-// pieces.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
+// Lane t of a quad holds ranks 8t .. 8t + 7 of each 32 (4t .. 4t + 3 of 16), and
+// columns 4t .. 4t + 3 of each 16 in two MMA tiles, so that B, base and out move
+// in 16-byte pieces.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
 // flight in a ring of its own, read back by the lanes that copied them.
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, 2)
     lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range) {
   using S = UpSmem<T, RK>;
-  constexpr int TM = S::TM, KS = RK / 16, PITCH = S::PITCH, PARTS = S::PARTS, D = S::kDepth;
+  constexpr int TM = S::TM, PITCH = S::PITCH, PARTS = S::PARTS, D = S::kDepth;
   __shared__ RowBlocks<TM> rb;
   __shared__ float undo[TM];
   extern __shared__ __align__(16) uint4 smem[];
@@ -372,7 +382,9 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
     }
   }
   __syncthreads();
-  uint2 w[4][KS];
+  constexpr int V = S::kVec, NVEC = RK / (4 * V);  // vectors of V ranks per lane
+  using Vec = std::conditional_t<V == 8, uint4, uint2>;
+  Vec w[4][NVEC];
   int held = -1, held_group = -1, group = 0, at = 0;
   for (int item = 0; item < items; ++item) {
     fetch(item + D - 1);
@@ -384,22 +396,23 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = c0 + 16 * (j >> 1) + 4 * (g >> 1) + 2 * (j & 1) + (g & 1);
+        const T *row = b + static_cast<long long>(c) * p.max_rank + V * t;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int r = 16 * k + 4 * t;
-          w[j][k] = make_uint2(0, 0);
-          if (c < p.n && r < rank) w[j][k] = *reinterpret_cast<const uint2 *>(b + static_cast<long long>(c) * p.max_rank + r);
+        for (int k = 0; k < NVEC; ++k) {
+          w[j][k] = Vec{};
+          if (c < p.n && 4 * V * k + V * t < rank) w[j][k] = *reinterpret_cast<const Vec *>(row + 4 * V * k);
         }
       }
-      if (rank % 4) {  // what lies past the rank may be anything
+      if (rank % V) {  // what lies past the rank may be anything
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const int left = rank - (16 * k + 4 * t);
-            if (left < 4) w[j][k].y &= left == 3 ? 0xffffu : 0u;
-            if (left < 2) w[j][k].x &= left == 1 ? 0xffffu : 0u;
-          }
+          for (int k = 0; k < NVEC; ++k)
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+              const int left = rank - (4 * V * k + V * t + 2 * e);
+              word(w[j][k], e) &= left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+            }
       }
     }
     if (++at == mine) at = 0, ++group;
@@ -418,15 +431,18 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       // places past the block's rows: those of other blocks, whose results are not stored
       const int r0 = min(start + g, TM - 1), r1 = min(start + g + 8, TM - 1);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        if (16 * k >= rank) break;
+      for (int k = 0; k < NVEC; ++k) {
+        if (4 * V * k >= rank) break;
 #pragma unroll
         for (int q = PARTS - 1; q >= 0; --q) {
-          const uint2 v0 = *reinterpret_cast<const uint2 *>(&ts[q][r0][16 * k + 4 * t]);
-          const uint2 v1 = *reinterpret_cast<const uint2 *>(&ts[q][r1][16 * k + 4 * t]);
-          const uint32_t a[4] = {v0.x, v1.x, v0.y, v1.y};
+          const Vec v0 = *reinterpret_cast<const Vec *>(&ts[q][r0][4 * V * k + V * t]);
+          const Vec v1 = *reinterpret_cast<const Vec *>(&ts[q][r1][4 * V * k + V * t]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_16<T>(acc[j], a, w[j][k].x, w[j][k].y);
+          for (int e = 0; e < V / 4; ++e) {
+            const uint32_t a[4] = {word(v0, 2 * e), word(v1, 2 * e), word(v0, 2 * e + 1), word(v1, 2 * e + 1)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_16<T>(acc[j], a, word(w[j][k], 2 * e), word(w[j][k], 2 * e + 1));
+          }
         }
       }
       const float down[2] = {undo[r0], undo[r1]};
