@@ -3,6 +3,7 @@
 //   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i . k_j + bias_j)
 //
 // in one pass over the keys with the running maximum and sum of the softmax.
+// Few rows: mma.sync, bound by the bytes of K and V.  Tiles of 128 rows: tcgen05.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -25,69 +26,6 @@ struct AttnArgs {
   int batch, q_len, kv_len, q_heads, group, dim;
   float scale;
 };
-
-constexpr int kRowWarps = 8;
-
-// One warp per query row: lanes split the head, every key is one dot product.
-template <typename T, typename TO>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_row_kernel(AttnArgs a) {
-  grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long long rows = static_cast<long long>(a.batch) * a.q_heads * a.q_len;
-  constexpr int kPer = kAttnMaxDim / 32;
-  for (long long r = static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); r < rows;
-       r += static_cast<long long>(gridDim.x) * kRowWarps) {
-    const long long i = r % a.q_len, h = r / a.q_len % a.q_heads, b = r / a.q_len / a.q_heads;
-    const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-    const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + h / a.group * a.ks[2];
-    const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + h / a.group * a.vs[2];
-    const int n = a.lens ? min(max(a.lens[b], 0), a.kv_len) : a.kv_len;
-    float qr[kPer], o[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int d = lane + 32 * j;
-      qr[j] = d < a.dim ? to_f32(q[d]) : 0.0f;
-      o[j] = 0.0f;
-    }
-    float top = -INFINITY, sum = 0.0f;
-    for (int t = 0; t < n; ++t) {
-      const float add = a.bias ? a.bias[b * a.bias_stride + t] : 0.0f;
-      if (add == -INFINITY) continue;
-      float s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int d = lane + 32 * j;
-        if (d < a.dim) s += qr[j] * to_f32(k[t * a.ks[1] + d]);
-      }
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-      s = s * a.scale + add;
-      const float m = fmaxf(top, s);
-      const float keep = m == top ? 1.0f : expf(top - m), p = expf(s - (m == -INFINITY ? 0.0f : m));
-      top = m;
-      sum = sum * keep + p;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int d = lane + 32 * j;
-        if (d < a.dim) o[j] = o[j] * keep + p * to_f32(v[t * a.vs[1] + d]);
-      }
-    }
-    TO *out = static_cast<TO *>(a.out) + b * a.os[0] + i * a.os[1] + h * a.os[2];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int d = lane + 32 * j;
-      if (d < a.dim) out[d] = from_f32<TO>(sum == 0.0f ? 0.0f : o[j] / sum);
-    }
-  }
-}
-
-template <typename T, typename TO>
-cudaError_t launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
-  const long long rows = static_cast<long long>(a.batch) * a.q_heads * a.q_len;
-  const long long blocks = (rows + kRowWarps - 1) / kRowWarps;
-  const unsigned grid = static_cast<unsigned>(blocks < 64LL * sms ? blocks : 64LL * sms);
-  return op_launch(attn_row_kernel<T, TO>, dim3(grid), kRowWarps * 32, 0, st, a);
-}
 
 // ------------------------------------------------------------ tiles of rows
 // 128 query rows of one head are one tile: S = Q K^T (128 rows x up to KT keys)
@@ -557,6 +495,272 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     out[d] = from_f32<TO>(sum == 0.0f ? 0.0f : o * inv);
   }
 }
+// ------------------------------------------------------------ few rows
+// Up to 16 query rows that share one key/value head (the tokens of a decode
+// step times the heads of a group): bound by reading K and V once.  Four warps
+// take every fourth chunk of 16 keys; each has a ring of chunks of its own,
+// filled by asynchronous copies, so about 100 KB are in flight per SM.  S and O
+// are m16n8k16 products on rows of the ring (ldmatrix, transposed for V), with
+// a running maximum and sum per warp, joined at the end through shared
+// memory, and over the key ranges of a unit by its last CTA, in order.  Keys
+// that take no part are never copied: their rows are zeros.
+constexpr int kFewWarps = 4, kFewRows = 16, kFewKeys = 16;
+
+struct FewArgs {
+  AttnArgs a;
+  int kv_heads, splits, per;  // per: chunks of one range
+  int unit16;                 // 16-byte pieces of a row in shared memory that hold data or zeros
+  uint32_t magic;             // i / unit16 = i * magic >> 16
+  float *part_o;              // [unit][split][16][dim]
+  float2 *part_ml;            // [unit][split][16]
+  uint32_t *counters;         // [unit], left zero
+};
+
+template <int DB>
+struct FewSmem {
+  static constexpr int kPitch = DB * 2 + 16;  // an odd number of 16-byte pieces: 8 rows on different banks
+  static constexpr int kStage = 2 * kFewKeys * kPitch;
+  static constexpr int kStages = DB == 64 ? 5 : DB == 128 ? 3 : 2;
+  static constexpr int kRing = kFewWarps * kStages * kStage;
+  static constexpr int kJoin = kFewWarps * kFewRows * (DB + 2) * 4;
+  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+
+template <typename T, typename TO, int DB>
+__global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __grid_constant__ FewArgs f) {
+  using S = FewSmem<DB>;
+  constexpr int KS = DB / 16, NS = S::kStages;
+  constexpr bool kParts = sizeof(TO) == 4;
+  constexpr float kShift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ bool last;
+  grid_dependency_wait();
+  const AttnArgs &a = f.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % f.splits, unit = blockIdx.x / f.splits;
+  const int kvh = unit % f.kv_heads, b = unit / f.kv_heads;
+  const int rows = a.q_len * a.group, n = clamped_len(a, b), dim = a.dim;
+  const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
+  const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
+  const float *bias = a.bias ? a.bias + b * a.bias_stride : nullptr;
+  const int chunks = (n + kFewKeys - 1) / kFewKeys;
+  const int first = min(split * f.per, chunks), end = min(first + f.per, chunks);
+
+  uint8_t *ring = smem + warp * (NS * S::kStage);
+  auto load = [&](int chunk, int slot) {
+    if (chunk < end) {
+      const int key0 = chunk * kFewKeys;
+      bool in = lane < kFewKeys && key0 + lane < n;
+      if (bias && in) in = ld_dep(bias + key0 + lane) != -INFINITY;
+      const uint32_t live = __ballot_sync(0xffffffffu, in);
+      uint8_t *ks = ring + slot * S::kStage, *vs = ks + kFewKeys * S::kPitch;
+      for (int i = lane; i < kFewKeys * f.unit16; i += 32) {
+        const int row = i * f.magic >> 16, piece = i - row * f.unit16;
+        const bool take = (live >> row & 1u) && piece * 8 < dim;
+        const long long key = take ? key0 + row : 0;
+        const int d = take ? piece * 8 : 0;
+        copy16(ks + row * S::kPitch + piece * 16, k + key * a.ks[1] + d, take);
+        copy16(vs + row * S::kPitch + piece * 16, v + key * a.vs[1] + d, take);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) load(first + warp + i * kFewWarps, i);
+
+  // the rows' queries as A operand: rows g and g + 8, elements 2t, 2t + 1 and 2t + 8, 2t + 9 of each 16
+  uint32_t q[KS][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = g + 8 * i;
+    const T *src = static_cast<const T *>(a.q) + b * a.qs[0] + static_cast<long long>(r < rows ? r / a.group : 0) * a.qs[1] +
+                   static_cast<long long>(kvh * a.group + (r < rows ? r % a.group : 0)) * a.qs[2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d = 16 * s + 8 * h + 2 * t;
+        q[s][2 * h + i] = r < rows && d < dim ? ld_dep(reinterpret_cast<const uint32_t *>(src + d)) : 0u;
+      }
+  }
+  const float c = a.scale * kLog2e;
+  float o[DB / 8][4];
+#pragma unroll
+  for (int j = 0; j < DB / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};  // of rows g, g + 8; sum: this lane's keys
+  int slot = 0;
+  for (int chunk = first + warp; chunk < end; chunk += kFewWarps) {
+    load(chunk + (NS - 1) * kFewWarps, slot == 0 ? NS - 1 : slot - 1);
+    copy_wait<NS - 1>();
+    __syncwarp();
+    const uint32_t ks = smem_u32(ring + slot * S::kStage), vs = ks + kFewKeys * S::kPitch;
+    slot = slot + 1 == NS ? 0 : slot + 1;
+    // s[h]: keys 8h + 2t, 8h + 2t + 1 of rows g (0, 1) and g + 8 (2, 3)
+    float s[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      if (16 * x >= dim) break;
+      // matrices: keys 0-7 and 8-15 of elements 0-7, then of 8-15
+      uint32_t m[4];
+      ldmatrix4(m, ks + (lane & 15) * S::kPitch + x * 32 + (lane >> 4) * 16);
+      mma_16<T>(s[0], q[x], m[0], m[2]);
+      mma_16<T>(s[1], q[x], m[1], m[3]);
+    }
+    const int key0 = chunk * kFewKeys;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int key = key0 + 8 * h + 2 * t + e;
+        float add = key < n ? 0.0f : -INFINITY;
+        if (bias && key < n) {
+          add = ld_dep(bias + key);
+          if (add != -INFINITY) add = fmaxf(add * kLog2e, -3.402823466e38f);  // the lowest finite bias stays finite
+        }
+        s[h][e] = add == -INFINITY ? -INFINITY : fmaf(s[h][e], c, add);
+        s[h][2 + e] = add == -INFINITY ? -INFINITY : fmaf(s[h][2 + e], c, add);
+      }
+    float keep[2];
+    bool moved = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float most = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const bool up = most > top[i];
+      keep[i] = up ? ex2_approx(top[i] - most) : 1.0f;
+      if (up) top[i] = most;
+      moved |= up;
+      sum[i] *= keep[i];
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int j = 0; j < DB / 8; ++j) o[j][0] *= keep[0], o[j][1] *= keep[0], o[j][2] *= keep[1], o[j][3] *= keep[1];
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float from = top[i] == -INFINITY ? 0.0f : top[i] - kShift;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float p0 = ex2_approx(s[h][2 * i] - from), p1 = ex2_approx(s[h][2 * i + 1] - from);
+        sum[i] += p0 + p1;
+        hi[2 * h + i] = pack2<T>(p0, p1);
+        if (kParts) {
+          const float2 back = unpack2<T>(hi[2 * h + i]);
+          lo[2 * h + i] = pack2<T>(p0 - back.x, p1 - back.y);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      if (16 * x >= dim) break;
+      // transposed matrices: keys 0-7 and 8-15 of elements 0-7, then of 8-15
+      uint32_t m[4];
+      ldmatrix4t(m, vs + (lane & 15) * S::kPitch + x * 32 + (lane >> 4) * 16);
+      if (kParts) mma_16<T>(o[2 * x], lo, m[0], m[1]);
+      mma_16<T>(o[2 * x], hi, m[0], m[1]);
+      if (kParts) mma_16<T>(o[2 * x + 1], lo, m[2], m[3]);
+      mma_16<T>(o[2 * x + 1], hi, m[2], m[3]);
+    }
+    __syncwarp();  // every lane is done with the chunk before its slot is filled again
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+  }
+  // join the warps: [warp][row][maximum, sum, dim sums]
+  __syncthreads();
+  float *join = reinterpret_cast<float *>(smem);
+  constexpr int kRow = DB + 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float *row = join + (warp * kFewRows + g + 8 * i) * kRow;
+    if (t == 0) row[0] = top[i], row[1] = sum[i];
+#pragma unroll
+    for (int j = 0; j < DB / 8; ++j)
+      *reinterpret_cast<float2 *>(row + 2 + 8 * j + 2 * t) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+  }
+  __syncthreads();
+  auto out_row = [&](int r) {
+    return static_cast<TO *>(a.out) + b * a.os[0] + static_cast<long long>(r / a.group) * a.os[1] +
+           static_cast<long long>(kvh * a.group + r % a.group) * a.os[2];
+  };
+  // one warp per row, lanes over the elements
+  for (int r = warp; r < rows; r += kFewWarps) {
+    float m = -INFINITY, l = 0.0f, w[kFewWarps];
+#pragma unroll
+    for (int x = 0; x < kFewWarps; ++x) m = fmaxf(m, join[(x * kFewRows + r) * kRow]);
+    const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int x = 0; x < kFewWarps; ++x) {
+      w[x] = ex2_approx(join[(x * kFewRows + r) * kRow] - from);
+      l += w[x] * join[(x * kFewRows + r) * kRow + 1];
+    }
+    const long long at = (static_cast<long long>(unit) * f.splits + split) * kFewRows + r;
+    for (int d = lane; d < dim; d += 32) {
+      float y = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kFewWarps; ++x) y += w[x] * join[(x * kFewRows + r) * kRow + 2 + d];
+      if (f.splits > 1)
+        f.part_o[at * dim + d] = y;
+      else
+        out_row(r)[d] = from_f32<TO>(l == 0.0f ? 0.0f : y / l);
+    }
+    if (f.splits > 1 && lane == 0) f.part_ml[at] = make_float2(m, l);
+  }
+  if (f.splits == 1) return;
+  // the unit's last CTA joins its ranges
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(f.counters + unit, 1u) == static_cast<uint32_t>(f.splits - 1);
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int r = warp; r < rows; r += kFewWarps) {
+    const long long at = static_cast<long long>(unit) * f.splits * kFewRows + r;
+    float m = -INFINITY, l = 0.0f;
+    for (int x = 0; x < f.splits; ++x) m = fmaxf(m, __ldcg(&f.part_ml[at + x * kFewRows].x));
+    const float from = m == -INFINITY ? 0.0f : m;
+    float y[DB / 32];
+#pragma unroll
+    for (int j = 0; j < DB / 32; ++j) y[j] = 0.0f;
+    for (int x = 0; x < f.splits; ++x) {
+      const float2 ml = __ldcg(&f.part_ml[at + x * kFewRows]);
+      const float w = ex2_approx(ml.x - from);
+      l += w * ml.y;
+#pragma unroll
+      for (int j = 0; j < DB / 32; ++j) {
+        const int d = lane + 32 * j;
+        if (d < dim) y[j] += w * __ldcg(&f.part_o[(at + x * kFewRows) * dim + d]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < DB / 32; ++j) {
+      const int d = lane + 32 * j;
+      if (d < dim) out_row(r)[d] = from_f32<TO>(l == 0.0f ? 0.0f : y[j] / l);
+    }
+  }
+  if (threadIdx.x == 0) f.counters[unit] = 0;
+}
+
 // A 4-D map {dim, tokens, heads, batch} of one operand, boxes of 64 x box_rows.
 // Heads or batches that share one copy (stride 0) become one; strides of
 // extents of one are not looked at.
@@ -623,9 +827,70 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   return op_result(e);
 }
 
+// No keys: every row is zero.
+__global__ void __launch_bounds__(256) attn_zero_kernel(AttnArgs a, int out_bytes) {
+  grid_dependency_wait();
+  const long long rows = static_cast<long long>(a.batch) * a.q_heads * a.q_len, total = rows * a.dim;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const long long row = i / a.dim, q = row % a.q_len, h = row / a.q_len % a.q_heads, b = row / a.q_len / a.q_heads;
+    const long long at = b * a.os[0] + q * a.os[1] + h * a.os[2] + i % a.dim;
+    if (out_bytes == 4)
+      static_cast<uint32_t *>(a.out)[at] = 0;
+    else
+      static_cast<uint16_t *>(a.out)[at] = 0;
+  }
+}
+
+template <typename T, typename TO, int DB>
+int run_few(const struct htpg_attention_params *p, const AttnArgs &a, const OpDevice &d, cudaStream_t st) {
+  using S = FewSmem<DB>;
+  FewArgs f = {};
+  f.a = a;
+  f.kv_heads = p->kv_heads;
+  f.unit16 = (a.dim + 15) / 16 * 2;
+  f.magic = (65536 + f.unit16 - 1) / f.unit16;
+  const long long units = static_cast<long long>(a.batch) * p->kv_heads;
+  if (units > (1 << 30)) return HTPG_ECAPACITY;
+  const int chunks = (a.kv_len + kFewKeys - 1) / kFewKeys;
+  // Key ranges: as many as make the rounds of CTAs (two per SM) shortest, a
+  // CTA's set-up and joining counted as two chunks per warp.
+  const long long slots = 2LL * d.sms;
+  f.splits = 1;
+  long long least = -1;
+  for (int s = 1; s <= 64 && (s == 1 || (units * s <= 4 * slots && s * kFewWarps <= chunks)); ++s) {
+    const int per = (chunks + s - 1) / s;
+    const long long cost = (units * s + slots - 1) / slots * ((per + kFewWarps - 1) / kFewWarps + 2);
+    if (least < 0 || cost < least) least = cost, f.splits = s;
+  }
+  f.per = (chunks + f.splits - 1) / f.splits;
+  std::unique_lock<std::mutex> lock;
+  if (f.splits > 1) {
+    lock = op_lock();
+    uint8_t *scratch;
+    const size_t ml = static_cast<size_t>(units) * f.splits * kFewRows * sizeof(float2);
+    const int rc = op_scratch(st, ml + static_cast<size_t>(units) * f.splits * kFewRows * a.dim * 4, &f.counters, &scratch);
+    if (rc) return rc;
+    f.part_ml = reinterpret_cast<float2 *>(scratch);
+    f.part_o = reinterpret_cast<float *>(scratch + ml);
+  }
+  auto *fn = attn_few_kernel<T, TO, DB>;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+  if (e != cudaSuccess) return op_result(e);
+  return op_result(op_launch(fn, dim3(static_cast<unsigned>(units * f.splits)), kFewWarps * 32, S::kBytes, st, f));
+}
+
 template <typename T, typename TO>
 int run_attention(const struct htpg_attention_params *p, const AttnArgs &a, const OpDevice &d, cudaStream_t st) {
-  if (a.q_len <= 16 || a.kv_len == 0) return op_result(launch_attn<T, TO>(a, d.sms, st));
+  if (a.kv_len == 0) {
+    const long long blocks = (static_cast<long long>(a.batch) * a.q_heads * a.q_len * a.dim + 255) / 256;
+    return op_result(op_launch(attn_zero_kernel, dim3(static_cast<unsigned>(std::min<long long>(blocks, 16LL * d.sms))), 256,
+                               0, st, a, static_cast<int>(sizeof(TO))));
+  }
+  if (static_cast<long long>(a.q_len) * a.group <= kFewRows) {
+    if (a.dim <= 64) return run_few<T, TO, 64>(p, a, d, st);
+    if (a.dim <= 128) return run_few<T, TO, 128>(p, a, d, st);
+    return run_few<T, TO, 192>(p, a, d, st);
+  }
   if (a.dim <= 64) return run_tiles<T, TO, 64, 128>(p, a, d, st);
   if (a.dim <= 128) return run_tiles<T, TO, 128, 128>(p, a, d, st);
   return run_tiles<T, TO, 192, 64>(p, a, d, st);
