@@ -54,7 +54,7 @@ struct TileArgs {
   int pairs;           // tile pairs of one key/value head: ceil(group * row_tiles / 2)
   int kv_heads;
   int splits;          // ranges of keys of one pair
-  long long items;     // batch * kv_heads * pairs * splits
+  int items;           // batch * kv_heads * pairs * splits
   int q_batch, k_batch, k_head, v_batch, v_head;  // 0: that dimension's stride is 0 (one copy)
   int wide;            // output rows are 32-byte aligned
   float *part_o;       // splits > 1: [splits][rows][dim] sums
@@ -69,7 +69,7 @@ struct TileSmem {
   static constexpr int kStage = KT * DP * 2;
   static constexpr int kStages = DP == 128 ? 4 : DP == 64 ? 6 : 5;
   static constexpr int kBars = 2 * kQ + kStages * kStage;
-  static constexpr int kLens = kBars + 8 * (2 + 2 * kStages + 7) + 24;
+  static constexpr int kLens = kBars + 8 * (2 * kStages + 11) + 24;
   static constexpr int kBias = (kLens + 4 * kLensHeld + 15) / 16 * 16;  // [tile][2][KT]
   static constexpr int kBytes = kBias + 16 * KT + 1024;                 // + alignment
 };
@@ -85,24 +85,29 @@ __device__ __forceinline__ int clamped_len(const AttnArgs &a, int b) {
 }
 
 template <int KT>
-__device__ __forceinline__ TileItem tile_item(const TileArgs &t, long long item, const int *lens) {
+__device__ __forceinline__ TileItem tile_item(const TileArgs &t, int item, const int *lens) {
   TileItem r;
-  r.split = static_cast<int>(item % t.splits);
-  long long u = item / t.splits;
-  const int pair = static_cast<int>(u % t.pairs);
-  u /= t.pairs;
-  r.kvh = static_cast<int>(u % t.kv_heads);
-  r.b = static_cast<int>(u / t.kv_heads);
+  uint32_t u = item, pair;
+  r.split = 0;
+  if (t.splits > 1) {
+    u = u / t.splits;
+    r.split = item - u * t.splits;
+  }
+  pair = u;
+  u = u / t.pairs;
+  pair -= u * t.pairs;
+  r.b = u / t.kv_heads;
+  r.kvh = u - r.b * t.kv_heads;
   r.n = r.b < kLensHeld ? lens[r.b] : clamped_len(t.a, r.b);
   const int tiles = (r.n + KT - 1) / KT, per = (tiles + t.splits - 1) / t.splits;
   r.j0 = min(r.split * per, tiles);
   r.j1 = min(r.j0 + per, tiles);
-  r.two = 2 * pair + 1 < t.a.group * t.row_tiles;
+  r.two = 2 * static_cast<int>(pair) + 1 < t.a.group * t.row_tiles;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int tile = 2 * pair + w;
-    r.head[w] = r.kvh * t.a.group + tile / t.row_tiles;
-    r.row0[w] = tile % t.row_tiles * 128;
+    const uint32_t tile = 2 * pair + w, head = t.a.group == 1 ? 0 : tile / t.row_tiles;
+    r.head[w] = r.kvh * t.a.group + head;
+    r.row0[w] = (tile - head * t.row_tiles) * 128;
   }
   return r;
 }
@@ -164,9 +169,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t *base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t q_s = smem_u32(base), kv_s = q_s + 2 * L::kQ;
   const uint32_t bars = q_s + L::kBars;
-  const uint32_t kv_full = bars, kv_empty = bars + 8 * NS, q_full = bars + 16 * NS, q_empty = q_full + 8;
-  const uint32_t s_full = q_empty + 8, p_ready = s_full + 16, o_full = p_ready + 16, mma_done = o_full + 16;
-  uint32_t *slot = reinterpret_cast<uint32_t *>(base + L::kBars + 8 * (2 * NS + 9));
+  const uint32_t kv_full = bars, kv_empty = bars + 8 * NS, q_full = bars + 16 * NS, q_empty = q_full + 16;
+  const uint32_t s_full = q_empty + 16, p_ready = s_full + 16, o_full = p_ready + 16, mma_done = o_full + 16;
+  uint32_t *slot = reinterpret_cast<uint32_t *>(base + L::kBars + 8 * (2 * NS + 11));
   volatile uint32_t *abort = slot + 1;
   int *lens = reinterpret_cast<int *>(base + L::kLens);
 
@@ -174,9 +179,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (threadIdx.x == 0) {
     *abort = 0;
     for (int i = 0; i < NS; ++i) mbar_init(kv_full + 8 * i, 1), mbar_init(kv_empty + 8 * i, 1);
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int w = 0; w < 2; ++w) {
+      mbar_init(q_full + 8 * w, 1);
+      mbar_init(q_empty + 8 * w, 1);
       mbar_init(s_full + 8 * w, 1);
       mbar_init(p_ready + 8 * w, 4);
       mbar_init(o_full + 8 * w, 1);
@@ -206,96 +211,116 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp == 9 && lane == 0) {
       // ------------------------------------------------------------ loads
       bool ok = true;
-      uint32_t loads = 0, tiles = 0;  // K and V tiles, query tile pairs issued
+      uint32_t loads = 0, tiles[2] = {0, 0};  // K and V tiles, query tiles issued
+      const int panels = (dim + 63) / 64;
       auto load = [&](const CUtensorMap *map, int j, int h, int b) {
         const uint32_t s = loads % NS, ph = loads / NS & 1u;
         if (!mbar_wait(kv_empty + 8 * s, ph ^ 1u, t.watchdog, kWatchProducer, abort)) return false;
-        mbar_arrive_expect_tx(kv_full + 8 * s, ((dim + 63) / 64) * KT * 128);
-        for (int p = 0; p * 64 < dim; ++p)
+        mbar_arrive_expect_tx(kv_full + 8 * s, panels * KT * 128);
+        for (int p = 0; p < panels; ++p)
           tma_load_4d(kv_s + s * L::kStage + p * KT * 128, map, kv_full + 8 * s, p * 64, j * KT, h, b);
         ++loads;
         return true;
       };
-      for (long long item = blockIdx.x; ok && item < t.items; item += gridDim.x) {
+      for (int item = blockIdx.x; ok && item < t.items; item += gridDim.x) {
         const TileItem it = tile_item<KT>(t, item, lens);
         if (it.j0 == it.j1) continue;
-        ok = mbar_wait(q_empty, (tiles & 1u) ^ 1u, t.watchdog, kWatchProducer, abort);
-        if (!ok) break;
-        const int panels = (dim + 63) / 64;
-        mbar_arrive_expect_tx(q_full, (it.two ? 2 : 1) * panels * 128 * 128);
-        for (int w = 0; w < (it.two ? 2 : 1); ++w)
+        for (int w = 0; ok && w < (it.two ? 2 : 1); ++w) {
+          ok = mbar_wait(q_empty + 8 * w, (tiles[w] & 1u) ^ 1u, t.watchdog, kWatchProducer, abort);
+          if (!ok) break;
+          mbar_arrive_expect_tx(q_full + 8 * w, panels * 128 * 128);
           for (int p = 0; p < panels; ++p)
-            tma_load_4d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full, p * 64, it.row0[w], it.head[w], it.b * t.q_batch);
-        ++tiles;
+            tma_load_4d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, it.row0[w], it.head[w],
+                        it.b * t.q_batch);
+          ++tiles[w];
+          // the first keys right after the first tile's queries
+          if (w == 0) ok = load(&map_k, it.j0, it.kvh * t.k_head, it.b * t.k_batch);
+        }
         for (int j = it.j0; ok && j < it.j1; ++j) {
-          ok = load(&map_k, j, it.kvh * t.k_head, it.b * t.k_batch);
+          if (j > it.j0) ok = load(&map_k, j, it.kvh * t.k_head, it.b * t.k_batch);
           ok = ok && load(&map_v, j, it.kvh * t.v_head, it.b * t.v_batch);
         }
       }
       // never leave the CTA with a copy still landing in its shared memory
       for (uint32_t i = loads > NS ? loads - NS : 0; i < loads; ++i)
         mbar_wait(kv_full + 8 * (i % NS), i / NS & 1u, t.watchdog, kWatchProducer, abort);
-      if (tiles) mbar_wait(q_full, (tiles - 1) & 1u, t.watchdog, kWatchProducer, abort);
+      for (int w = 0; w < 2; ++w)
+        if (tiles[w]) mbar_wait(q_full + 8 * w, (tiles[w] - 1) & 1u, t.watchdog, kWatchProducer, abort);
     }
     if (warp == 8 && lane == 0) {
       // ------------------------------------------------------------- MMAs
-      bool ok = true;
-      uint32_t used = 0, tiles = 0, ready[2] = {0, 0};
       const int ksteps = (dim + 15) / 16;
+      const uint64_t desc_q = umma_desc_sw128(q_s), desc_k = umma_desc_sw128(kv_s), desc_v = umma_desc_sw128_mn(kv_s, KT * 128);
       const uint32_t idesc_v = kIdesc | (1u << 16) | (static_cast<uint32_t>(ksteps * 2) << 17);  // V: MN-major, N = dim
       auto wait = [&](uint32_t bar, uint32_t parity) {
         const bool got = mbar_wait(bar, parity, t.watchdog, kWatchMma, abort);
         tc_fence_after();
         return got;
       };
-      // S of tile w = Q K^T with the key tile in slot `u`
-      auto scores = [&](int w, uint32_t u, int keys) {
-        const uint32_t k_at = kv_s + (u % NS) * L::kStage, q_at = q_s + w * L::kQ;
-        const uint32_t idesc = kIdesc | (static_cast<uint32_t>((keys + 15) / 16 * 2) << 17);
-        for (int i = 0; i < ksteps; ++i)
-          umma_f16(tmem + w * KT, umma_desc_sw128(q_at + i / 4 * 128 * 128 + i % 4 * 32),
-                   umma_desc_sw128(k_at + i / 4 * KT * 128 + i % 4 * 32), idesc, i > 0);
-        tc_commit(s_full + 8 * w);
-      };
-      for (long long item = blockIdx.x; ok && item < t.items; item += gridDim.x) {
-        const TileItem it = tile_item<KT>(t, item, lens);
-        const int nt = it.j1 - it.j0, nw = it.two ? 2 : 1;
-        if (!nt) continue;
-        ok = wait(q_full, tiles & 1u) && wait(kv_full + 8 * (used % NS), used / NS & 1u);
-        if (!ok) break;
-        ++tiles;
-        for (int w = 0; w < nw; ++w) scores(w, used, min(KT, it.n - it.j0 * KT));
-        tc_commit(kv_empty + 8 * (used % NS));
-        if (nt == 1) tc_commit(q_empty);
-        for (int j = 0; ok && j < nt; ++j) {
-          // slots: key tile j = used, value tile j = used + 1, key tile j + 1 = used + 2
-          const int keys = min(KT, it.n - (it.j0 + j) * KT);
-          const uint32_t v_slot = (used + 1) % NS;
-          for (int w = 0; ok && w < nw; ++w) {
-            ok = wait(p_ready + 8 * w, ready[w]++ & 1u);
-            if (ok && w == 0) ok = wait(kv_full + 8 * v_slot, (used + 1) / NS & 1u);
-            if (!ok) break;
-            const int vsteps = (keys + 15) / 16;
-            for (int part = 0; part < (kParts ? 2 : 1); ++part)
-              for (int i = 0; i < vsteps; ++i)
-                umma_f16_ta(tmem + kO + w * DP, tmem + w * KT + part * (KT / 2) + i * 8,
-                            umma_desc_sw128_mn(kv_s + v_slot * L::kStage + i * 2048, KT * 128), idesc_v,
-                            j > 0 || part > 0 || i > 0);
-            if (w == nw - 1) tc_commit(kv_empty + 8 * v_slot);
-            if (j + 1 < nt) {
-              if (w == 0) ok = wait(kv_full + 8 * ((used + 2) % NS), (used + 2) / NS & 1u);
-              if (!ok) break;
-              scores(w, used + 2, min(KT, it.n - (it.j0 + j + 1) * KT));
-              if (w == nw - 1) {
-                tc_commit(kv_empty + 8 * ((used + 2) % NS));
-                if (j + 2 == nt) tc_commit(q_empty);
-              }
-            } else {
-              tc_commit(o_full + 8 * w);
-            }
-          }
-          used += 2;
+      // Steps: the key tiles of this CTA's items, one after the other.  At each,
+      // tile by tile: O += P V of the step before, then S = Q K^T of this one, so
+      // that a tile's next scores (of the next item, too) are under way while the
+      // other tile's weights are still being made.  Slots: K of step n in 2n, V in 2n + 1.
+      struct Step {
+        int tiles = 0, keys = 0;
+        bool first = false, last = false;
+      } now, before;
+      uint32_t queries[2] = {0, 0}, ready[2] = {0, 0}, n = 0;
+      TileItem it;
+      int item = blockIdx.x, j = 0;
+      bool ok = true, open = false;
+      for (; ok; ++n) {
+        // the next step
+        now.tiles = 0;
+        while (!open && item < t.items) {
+          it = tile_item<KT>(t, item, lens);
+          item += gridDim.x;
+          j = it.j0;
+          open = it.j0 < it.j1;
         }
+        if (open) {
+          now.tiles = it.two ? 2 : 1;
+          now.keys = min(KT, it.n - j * KT);
+          now.first = j == it.j0;
+          now.last = ++j == it.j1;
+          open = !now.last;
+        }
+        if (!now.tiles && !before.tiles) break;
+        const uint32_t k_slot = 2 * n % NS, v_slot = (2 * n - 1) % NS;  // v_slot: of the step before
+        for (int w = 0; ok && w < 2; ++w) {
+          if (w < before.tiles) {
+            ok = wait(p_ready + 8 * w, ready[w]++ & 1u);
+            if (ok && w == 0) ok = wait(kv_full + 8 * v_slot, (2 * n - 1) / NS & 1u);
+            if (!ok) break;
+            const int vsteps = (before.keys + 15) / 16;
+            const uint64_t dv = desc_v + v_slot * (L::kStage / 16);
+            uint32_t more = !before.first;  // 0: O is overwritten
+#pragma unroll
+            for (int part = 0; part < (kParts ? 2 : 1); ++part) {
+              const uint32_t o_t = tmem + kO + w * DP, p_t = tmem + w * KT + part * (KT / 2);
+              int i = 0;
+              for (; i + 4 <= vsteps; i += 4, more = 1) umma_f16_ta4(o_t, p_t + i * 8, dv + i * 128, 128, idesc_v, more);
+              for (; i < vsteps; ++i, more = 1) umma_f16_ta(o_t, p_t + i * 8, dv + i * 128, idesc_v, more);
+            }
+            if (before.last) tc_commit(o_full + 8 * w);
+            if (w == before.tiles - 1) tc_commit(kv_empty + 8 * v_slot);
+          }
+          if (w < now.tiles) {
+            if (now.first) ok = wait(q_full + 8 * w, queries[w]++ & 1u);
+            if (ok && w == 0) ok = wait(kv_full + 8 * k_slot, 2 * n / NS & 1u);
+            if (!ok) break;
+            uint64_t dq = desc_q + w * (L::kQ / 16), dk = desc_k + k_slot * (L::kStage / 16);
+            const uint32_t idesc = kIdesc | (static_cast<uint32_t>((now.keys + 15) / 16 * 2) << 17);
+            int i = 0;
+            for (; i + 4 <= ksteps; i += 4, dq += 128 * 128 / 16, dk += KT * 128 / 16)
+              umma_f16_kblock(tmem + w * KT, dq, dk, idesc, i > 0);
+            for (; i < ksteps; ++i, dq += 2, dk += 2) umma_f16(tmem + w * KT, dq, dk, idesc, i > 0);
+            tc_commit(s_full + 8 * w);
+            if (w == now.tiles - 1) tc_commit(kv_empty + 8 * k_slot);
+            if (now.last) tc_commit(q_empty + 8 * w);
+          }
+        }
+        before = now;
       }
       tc_commit(mma_done);  // every MMA is complete before TMEM is freed
       mbar_wait(mma_done, 0, t.watchdog, kWatchMma, abort);
@@ -318,7 +343,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     };
     // No early exit: a tile's threads meet at its named barriers in every
     // iteration; after a wait that gave up they skip the work.
-    for (long long item = blockIdx.x; item < t.items; item += gridDim.x) {
+    for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
       const TileItem it = tile_item<KT>(t, item, lens);
       const int nt = it.j1 - it.j0;
       if (w == 1 && !it.two) {
@@ -343,28 +368,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         ok = wait(ok, s_full + 8 * w, seen++ & 1u);
         if (!ok) continue;
-        float s[KT / 32][32];
+        // What takes no part becomes -inf; with a bias scores are in units of
+        // log2.  Four running maxima and sums: one of each would be a chain of
+        // 128 dependent operations.
+        float2 s[KT / 32][16];
+        float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int g = 0; g < KT / 32; ++g)
-          if (g * 32 < keys) tmem_ld32(s_at + g * 32, s[g]);
+        for (int c32 = 0; c32 < KT / 32; ++c32)
+          if (c32 * 32 < keys) tmem_ld32(s_at + c32 * 32, s[c32]);
         tmem_ld_wait();
-        // what takes no part becomes -inf; with a bias scores are in units of log2
-        if (bias) {
-          const float *add = bias_s + (j & 1) * KT;
 #pragma unroll
-          for (int i = 0; i < KT; ++i) {
-            const float x = add[i];
-            s[i / 32][i % 32] = x == -INFINITY ? -INFINITY : fmaf(s[i / 32][i % 32], c, x);
+        for (int c32 = 0; c32 < KT / 32; ++c32) {
+          if (c32 * 32 >= keys) break;
+          if (bias) {
+            const float4 *add = reinterpret_cast<const float4 *>(bias_s + (j & 1) * KT + c32 * 32);
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) {
+              const float4 y = add[x / 2];
+              const float2 f0 = fma2(s[c32][x], make_float2(c, c), make_float2(y.x, y.y));
+              const float2 f1 = fma2(s[c32][x + 1], make_float2(c, c), make_float2(y.z, y.w));
+              s[c32][x] = make_float2(y.x == -INFINITY ? -INFINITY : f0.x, y.y == -INFINITY ? -INFINITY : f0.y);
+              s[c32][x + 1] = make_float2(y.z == -INFINITY ? -INFINITY : f1.x, y.w == -INFINITY ? -INFINITY : f1.y);
+            }
+          } else if (c32 * 32 + 32 > keys) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              if (c32 * 32 + 2 * x >= keys) s[c32][x].x = -INFINITY;
+              if (c32 * 32 + 2 * x + 1 >= keys) s[c32][x].y = -INFINITY;
+            }
           }
-        } else if (keys < KT) {
 #pragma unroll
-          for (int i = 0; i < KT; ++i)
-            if (i >= keys) s[i / 32][i % 32] = -INFINITY;
+          for (int x = 0; x < 16; ++x) most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[c32][x].x, s[c32][x].y));
         }
-        float most = s[0][0];
-#pragma unroll
-        for (int i = 1; i < KT; ++i) most = fmaxf(most, s[i / 32][i % 32]);
-        most *= unit;
+        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3])) * unit;
         const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
           const float keep = raise ? ex2_approx(top - most) : 1.0f;
@@ -374,40 +410,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           if (j > 0) {
             // the tensor core is done with O: S of this tile came after it
+#pragma unroll 1
+            for (int i = 0; i < dim; i += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_at + i, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < DP; i += 32) {
-              if (i < dim) {
-                uint32_t o[32];
-                tmem_ld32(o_at + i, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
-                tmem_st32(o_at + i, o);
-              }
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+              tmem_st32(o_at + i, o);
             }
           }
         }
         const float from = top == -INFINITY ? 0.0f : top - kShift;
+        float2 sum4[4] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-        for (int g = 0; g < KT / 32; ++g) {
-          if (g * 32 < keys) {
-            uint32_t hi[16], lo[16];
+        for (int c32 = 0; c32 < KT / 32; ++c32) {
+          if (c32 * 32 >= keys) break;
+          uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const float p0 = ex2_approx(fmaf(s[g][2 * x], unit, -from));
-              const float p1 = ex2_approx(fmaf(s[g][2 * x + 1], unit, -from));
-              sum += p0;
-              sum += p1;
-              hi[x] = pack2<T>(p0, p1);
-              if (kParts) {
-                const float2 back = unpack2<T>(hi[x]);
-                lo[x] = pack2<T>(p0 - back.x, p1 - back.y);
-              }
+          for (int x = 0; x < 16; ++x) {
+            float2 p = fma2(s[c32][x], make_float2(unit, unit), make_float2(-from, -from));
+            p = make_float2(ex2_approx(p.x), ex2_approx(p.y));
+            sum4[x % 4] = add2(sum4[x % 4], p);
+            hi[x] = pack2<T>(p.x, p.y);
+            if (kParts) {
+              const float2 back = unpack2<T>(hi[x]);
+              lo[x] = pack2<T>(p.x - back.x, p.y - back.y);
             }
-            tmem_st16(s_at + g * 16, hi);
-            if (kParts) tmem_st16(s_at + KT / 2 + g * 16, lo);
           }
+          tmem_st16(s_at + c32 * 16, hi);
+          if (kParts) tmem_st16(s_at + KT / 2 + c32 * 16, lo);
         }
+        sum4[0] = add2(add2(sum4[0], sum4[1]), add2(sum4[2], sum4[3]));
+        sum = sum4[0].x + sum4[0].y;
         tmem_st_wait();
         tc_fence_before();
         // Values of keys that take no part may be infinite or NaN, which a
@@ -433,28 +468,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (nt) ok = wait(ok, o_full + 8 * w, done++ & 1u);
       if (!ok) continue;
-      const float inv = t.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-      const bool none = sum == 0.0f;
+      const bool none = sum == 0.0f;  // then O is zero, or there was no tile
+      const float inv = t.splits > 1 || none ? 1.0f : 1.0f / sum;
       const long long row = (static_cast<long long>(it.b) * t.a.q_heads + it.head[w]) * t.a.q_len + it.row0[w] + r;
       TO *out = static_cast<TO *>(t.a.out) + it.b * t.a.os[0] + static_cast<long long>(it.row0[w] + r) * t.a.os[1] +
                 it.head[w] * t.a.os[2];
       float *part = t.splits > 1 ? t.part_o + (it.split * t.rows + row) * dim : nullptr;
+#pragma unroll 1
+      for (int i = 0; i < dim; i += 32) {
+        float o[32];
+        if (nt) {
+          tmem_ld32(o_at + i, o);
+          tmem_ld_wait();
+        }
 #pragma unroll
-      for (int i = 0; i < DP; i += 32) {
-        if (i < dim) {
-          float o[32];
-          if (nt) {
-            tmem_ld32(o_at + i, o);
-            tmem_ld_wait();
-          }
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = none ? 0.0f : o[x] * inv;
-          if (mine) {
-            if (part)
-              store_columns<float>(part, i, dim, o, true);
-            else
-              store_columns<TO>(out, i, dim, o, wide);
-          }
+        for (int x = 0; x < 32; ++x) o[x] = nt ? o[x] * inv : 0.0f;
+        if (mine) {
+          if (part)
+            store_columns<float>(part, i, dim, o, true);
+          else
+            store_columns<TO>(out, i, dim, o, wide);
         }
       }
       if (part && mine) t.part_ml[it.split * t.rows + row] = make_float2(none ? -INFINITY : top, sum);
@@ -793,7 +826,8 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   const int tiles = (a.kv_len + KT - 1) / KT;
   t.splits = 1;
   if (units * 2 <= d.sms && tiles >= 4) t.splits = static_cast<int>(std::min<long long>(d.sms / units, tiles / 2));
-  t.items = units * t.splits;
+  if (units * t.splits > 0x3fffffff) return HTPG_ECAPACITY;
+  t.items = static_cast<int>(units * t.splits);
   t.wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
   const int qe[3] = {a.batch, a.q_len, a.q_heads};
   for (int i = 0; i < 3; ++i)
@@ -820,7 +854,7 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   using L = TileSmem<DP, KT>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return op_result(e);
-  e = op_launch(fn, dim3(static_cast<unsigned>(std::min<long long>(t.items, d.sms))), kTileThreads, L::kBytes, st, mq, mk,
+  e = op_launch(fn, dim3(static_cast<unsigned>(std::min(t.items, d.sms))), kTileThreads, L::kBytes, st, mq, mk,
                 mv, t);
   if (e == cudaSuccess && t.splits > 1)
     e = op_launch(attn_join_kernel<TO>, dim3(static_cast<unsigned>((t.rows + 7) / 8)), 256, 0, st, t);

@@ -110,16 +110,6 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_row_kernel(RopeArgs a) {
 }
 
 // ---------------------------------------------------------------- vectors
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
-  return reinterpret_cast<float2 &>(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
-  return reinterpret_cast<float2 &>(r);
-}
 // N consecutive elements as FP32 (ONCE: evicted first), and back.
 template <typename T, int N, bool ONCE = true>
 __device__ __forceinline__ void load_n(const T *p, float *v) {
