@@ -28,21 +28,22 @@ struct AttnArgs {
 };
 
 // ------------------------------------------------------------ tiles of rows
-// 128 query rows of one head are one tile: S = Q K^T (128 rows x up to KT keys)
+// 128 query rows of one head are one tile: S = Q K^T (128 rows x up to 64 keys)
 // and O += P V are tcgen05.mma into TMEM, softmax in registers, one thread per
 // row.  A CTA holds two tiles that share their keys and values (neighbouring
-// rows of one head, or heads of one group), so that the tensor core works for
-// one while the other's softmax runs:
+// rows of one head, or heads of one group):
 //   warps 0-3, 4-7  softmax of tile 0, 1: S from TMEM, running maximum and sum,
 //                   P (16 bits) back into TMEM over S, and the tile's output
-//   warp 8          issues the MMAs, warp 9 the TMA loads (10 and 11 only make
-//                   the warpgroup whole, to hand its registers to the others:
+//   warps 8, 10     issue the MMAs of tile 0, 1; warp 9 the TMA loads (11 only
+//                   makes the warpgroup whole, to hand its registers to the others:
 //                   256 x 216 + 128 x 72 = 384 x 168, what the launch gives)
-// TMEM columns: S of tile 0 and 1 (KT each, P in place), O of both (DP each).
-// P is the A operand in TMEM; V, as loaded ([key][dim]), the MN-major B operand.
-// The maximum is only raised (and O rescaled) once a score passes it by 2^8:
-// weights up to 2^8 (FP16: 2^15, see kShift) stay exact enough and most tiles
-// skip the rescale.
+// TMEM columns: per tile two buffers of S (64 each, P in place; one buffer for
+// heads above 128) and O (DP).  With two, the scores of the next two key tiles are
+// made while the softmax of one runs, so the chain scores -> softmax -> weights
+// never waits for the tensor core.  P is the A operand in TMEM; V, as loaded ([key][dim]), the
+// MN-major B operand.  The maximum is only raised (and O rescaled) once a score
+// passes it by 2^8: weights up to 2^8 (FP16: 2^15, see kShift) stay exact
+// enough and most tiles skip the rescale.
 constexpr int kTileThreads = 384;
 constexpr int kLensHeld = 256;   // batches whose lengths are kept in shared memory
 constexpr float kLazy = 8.0f;    // log2 of how far a score may pass the held maximum
@@ -67,9 +68,11 @@ template <int DP, int KT>
 struct TileSmem {
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kStage = KT * DP * 2;
-  static constexpr int kStages = DP == 128 ? 4 : DP == 64 ? 6 : 5;
+  static constexpr int kStages = DP == 128 ? 8 : DP == 64 ? 10 : 5;
+  static constexpr int kBuffers = DP == 192 ? 1 : 2;  // of S, per tile
+  static constexpr int kBarriers = 2 * kStages + 18;
   static constexpr int kBars = 2 * kQ + kStages * kStage;
-  static constexpr int kLens = kBars + 8 * (2 * kStages + 11) + 24;
+  static constexpr int kLens = kBars + 8 * kBarriers + 24;
   static constexpr int kBias = (kLens + 4 * kLensHeld + 15) / 16 * 16;  // [tile][2][KT]
   static constexpr int kBytes = kBias + 16 * KT + 1024;                 // + alignment
 };
@@ -163,30 +166,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr uint32_t kFormat = std::is_same<T, __half>::value ? 0u : 1u;
   constexpr uint32_t kIdesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | (8u << 24);  // F32 sums, M = 128
   constexpr int NS = L::kStages;
-  constexpr uint32_t kO = 2 * KT;  // first TMEM column of O
+  constexpr int NB = L::kBuffers;
+  constexpr uint32_t kO = 2 * NB * KT;  // first TMEM column of O
 
   extern __shared__ uint8_t raw[];
   uint8_t *base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t q_s = smem_u32(base), kv_s = q_s + 2 * L::kQ;
   const uint32_t bars = q_s + L::kBars;
   const uint32_t kv_full = bars, kv_empty = bars + 8 * NS, q_full = bars + 16 * NS, q_empty = q_full + 16;
-  const uint32_t s_full = q_empty + 16, p_ready = s_full + 16, o_full = p_ready + 16, mma_done = o_full + 16;
-  uint32_t *slot = reinterpret_cast<uint32_t *>(base + L::kBars + 8 * (2 * NS + 11));
+  // per tile and buffer; per tile
+  const uint32_t s_full = q_empty + 16, p_ready = s_full + 32, pv_done = p_ready + 32, mma_done = pv_done + 32;
+  uint32_t *slot = reinterpret_cast<uint32_t *>(base + L::kBars + 8 * L::kBarriers);
   volatile uint32_t *abort = slot + 1;
   int *lens = reinterpret_cast<int *>(base + L::kLens);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     *abort = 0;
-    for (int i = 0; i < NS; ++i) mbar_init(kv_full + 8 * i, 1), mbar_init(kv_empty + 8 * i, 1);
+    for (int i = 0; i < NS; ++i) mbar_init(kv_full + 8 * i, 1), mbar_init(kv_empty + 8 * i, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(q_full + 8 * w, 1);
       mbar_init(q_empty + 8 * w, 1);
-      mbar_init(s_full + 8 * w, 1);
-      mbar_init(p_ready + 8 * w, 4);
-      mbar_init(o_full + 8 * w, 1);
+      // (one of each per buffer: a wait for step n then cannot take step n - 1's phase for its own)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full + 16 * w + 8 * i, 1);
+        mbar_init(p_ready + 16 * w + 8 * i, 4);
+        mbar_init(pv_done + 16 * w + 8 * i, 1);
+      }
+      mbar_init(mma_done + 8 * w, 1);
     }
-    mbar_init(mma_done, 1);
     fence_barrier_init();
   }
   if (warp == 8) {
@@ -247,94 +255,129 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int w = 0; w < 2; ++w)
         if (tiles[w]) mbar_wait(q_full + 8 * w, (tiles[w] - 1) & 1u, t.watchdog, kWatchProducer, abort);
     }
-    if (warp == 8 && lane == 0) {
+    if (warp == 8 || warp == 10) {
       // ------------------------------------------------------------- MMAs
+      // The whole warp runs the loop, so that descriptors stay in uniform
+      // registers; lane 0 issues.
+      const int w = warp == 10;
       const int ksteps = (dim + 15) / 16;
-      const uint64_t desc_q = umma_desc_sw128(q_s), desc_k = umma_desc_sw128(kv_s), desc_v = umma_desc_sw128_mn(kv_s, KT * 128);
+      const uint64_t desc_q = umma_desc_sw128(q_s + w * L::kQ), desc_k = umma_desc_sw128(kv_s);
+      const uint64_t desc_v = umma_desc_sw128_mn(kv_s, KT * 128);
       const uint32_t idesc_v = kIdesc | (1u << 16) | (static_cast<uint32_t>(ksteps * 2) << 17);  // V: MN-major, N = dim
+      const uint32_t s_t = tmem + w * NB * KT, o_t = tmem + kO + w * DP;
       auto wait = [&](uint32_t bar, uint32_t parity) {
         const bool got = mbar_wait(bar, parity, t.watchdog, kWatchMma, abort);
         tc_fence_after();
-        return got;
+        return __all_sync(0xffffffffu, got) != 0;
       };
-      // Steps: the key tiles of this CTA's items, one after the other.  At each,
-      // tile by tile: O += P V of the step before, then S = Q K^T of this one, so
-      // that a tile's next scores (of the next item, too) are under way while the
-      // other tile's weights are still being made.  Slots: K of step n in 2n, V in 2n + 1.
+      // Steps: the key tiles of this CTA's items, one after the other.  At each:
+      // O += P V of the step NB before, then S = Q K^T of this one into the buffer
+      // that frees.  Slots: K of step n in 2n, V in 2n + 1; both tiles' warps
+      // release them, this one at once where the item has no second tile.
       struct Step {
-        int tiles = 0, keys = 0;
-        bool first = false, last = false;
-      } now, before;
-      uint32_t queries[2] = {0, 0}, ready[2] = {0, 0}, n = 0;
+        int keys = 0;  // 0: none
+        bool mine = false, first = false, last = false;
+      } past[NB];
+      uint32_t queries = 0, made = 0, taken = 0, n = 0;  // made, taken: steps of this tile
       TileItem it;
       int item = blockIdx.x, j = 0;
       bool ok = true, open = false;
       for (; ok; ++n) {
-        // the next step
-        now.tiles = 0;
+        Step now;
         while (!open && item < t.items) {
           it = tile_item<KT>(t, item, lens);
+          it.n = __shfl_sync(0xffffffffu, it.n, 0);
+          it.j0 = __shfl_sync(0xffffffffu, it.j0, 0);
+          it.j1 = __shfl_sync(0xffffffffu, it.j1, 0);
           item += gridDim.x;
           j = it.j0;
           open = it.j0 < it.j1;
         }
         if (open) {
-          now.tiles = it.two ? 2 : 1;
           now.keys = min(KT, it.n - j * KT);
+          now.mine = w == 0 || it.two;
           now.first = j == it.j0;
           now.last = ++j == it.j1;
           open = !now.last;
         }
-        if (!now.tiles && !before.tiles) break;
-        const uint32_t k_slot = 2 * n % NS, v_slot = (2 * n - 1) % NS;  // v_slot: of the step before
-        for (int w = 0; ok && w < 2; ++w) {
-          if (w < before.tiles) {
-            ok = wait(p_ready + 8 * w, ready[w]++ & 1u);
-            if (ok && w == 0) ok = wait(kv_full + 8 * v_slot, (2 * n - 1) / NS & 1u);
-            if (!ok) break;
-            const int vsteps = (before.keys + 15) / 16;
-            const uint64_t dv = desc_v + v_slot * (L::kStage / 16);
-            uint32_t more = !before.first;  // 0: O is overwritten
+        const Step old = past[0];
+        if (!now.keys && !old.keys && (NB == 1 || !past[NB - 1].keys)) break;
+        if (old.keys) {
+          const uint32_t v_slot = (2 * (n - NB) + 1) % NS, v_phase = (2 * (n - NB) + 1) / NS & 1u;
+          const uint32_t buf = taken % NB;
+          if (old.mine) ok = wait(p_ready + 16 * w + 8 * buf, taken / NB & 1u);
+          ok = ok && wait(kv_full + 8 * v_slot, v_phase);
+          if (!ok) break;
+          if (!old.mine) {
+            if (lane == 0) mbar_arrive(kv_empty + 8 * v_slot);
+          } else {
+            ++taken;
+            if (lane == 0) {
+              // P of 32 keys (two K = 16 steps): 16 columns high parts, 16 low, where their scores were
+              const uint64_t dv = desc_v + v_slot * (L::kStage / 16);
+              const uint32_t p_t = s_t + buf * KT;
+              uint32_t more = !old.first;  // 0: O is overwritten
 #pragma unroll
-            for (int part = 0; part < (kParts ? 2 : 1); ++part) {
-              const uint32_t o_t = tmem + kO + w * DP, p_t = tmem + w * KT + part * (KT / 2);
-              int i = 0;
-              for (; i + 4 <= vsteps; i += 4, more = 1) umma_f16_ta4(o_t, p_t + i * 8, dv + i * 128, 128, idesc_v, more);
-              for (; i < vsteps; ++i, more = 1) umma_f16_ta(o_t, p_t + i * 8, dv + i * 128, idesc_v, more);
+              for (int i = 0; i < KT / 32; ++i) {
+                if (i * 32 >= old.keys) break;
+                umma_f16_ta(o_t, p_t + i * 32, dv + i * 256, idesc_v, more);
+                if (kParts) umma_f16_ta(o_t, p_t + i * 32 + 16, dv + i * 256, idesc_v, 1);
+                more = 1;
+                if (i * 32 + 16 < old.keys) {
+                  umma_f16_ta(o_t, p_t + i * 32 + 8, dv + i * 256 + 128, idesc_v, 1);
+                  if (kParts) umma_f16_ta(o_t, p_t + i * 32 + 24, dv + i * 256 + 128, idesc_v, 1);
+                }
+              }
+              tc_commit(pv_done + 16 * w + 8 * buf);
+              tc_commit(kv_empty + 8 * v_slot);
             }
-            if (before.last) tc_commit(o_full + 8 * w);
-            if (w == before.tiles - 1) tc_commit(kv_empty + 8 * v_slot);
-          }
-          if (w < now.tiles) {
-            if (now.first) ok = wait(q_full + 8 * w, queries[w]++ & 1u);
-            if (ok && w == 0) ok = wait(kv_full + 8 * k_slot, 2 * n / NS & 1u);
-            if (!ok) break;
-            uint64_t dq = desc_q + w * (L::kQ / 16), dk = desc_k + k_slot * (L::kStage / 16);
-            const uint32_t idesc = kIdesc | (static_cast<uint32_t>((now.keys + 15) / 16 * 2) << 17);
-            int i = 0;
-            for (; i + 4 <= ksteps; i += 4, dq += 128 * 128 / 16, dk += KT * 128 / 16)
-              umma_f16_kblock(tmem + w * KT, dq, dk, idesc, i > 0);
-            for (; i < ksteps; ++i, dq += 2, dk += 2) umma_f16(tmem + w * KT, dq, dk, idesc, i > 0);
-            tc_commit(s_full + 8 * w);
-            if (w == now.tiles - 1) tc_commit(kv_empty + 8 * k_slot);
-            if (now.last) tc_commit(q_empty + 8 * w);
           }
         }
-        before = now;
+        if (now.keys) {
+          const uint32_t k_slot = 2 * n % NS;
+          if (now.mine && now.first) ok = wait(q_full + 8 * w, queries++ & 1u);
+          ok = ok && wait(kv_full + 8 * k_slot, 2 * n / NS & 1u);
+          if (!ok) break;
+          if (!now.mine) {
+            if (lane == 0) mbar_arrive(kv_empty + 8 * k_slot);
+          } else {
+            const uint32_t buf = made++ % NB;
+            if (lane == 0) {
+              uint64_t dq = desc_q, dk = desc_k + k_slot * (L::kStage / 16);
+              const uint32_t idesc = kIdesc | (static_cast<uint32_t>((now.keys + 15) / 16 * 2) << 17);
+              int i = 0;
+#pragma unroll
+              for (int panel = 0; panel < DP / 64; ++panel) {
+                if (i + 4 > ksteps) break;
+                umma_f16_kblock(s_t + buf * KT, dq, dk, idesc, i > 0);
+                i += 4, dq += 128 * 128 / 16, dk += KT * 128 / 16;
+              }
+#pragma unroll 1
+              for (; i < ksteps; ++i, dq += 2, dk += 2) umma_f16(s_t + buf * KT, dq, dk, idesc, i > 0);
+              tc_commit(s_full + 16 * w + 8 * buf);
+              tc_commit(kv_empty + 8 * k_slot);
+              if (now.last) tc_commit(q_empty + 8 * w);
+            }
+          }
+        }
+        if (NB > 1) past[0] = past[NB - 1];
+        past[NB - 1] = now;
       }
-      tc_commit(mma_done);  // every MMA is complete before TMEM is freed
-      mbar_wait(mma_done, 0, t.watchdog, kWatchMma, abort);
+      if (lane == 0) {
+        tc_commit(mma_done + 8 * w);  // every MMA is complete before TMEM is freed
+        mbar_wait(mma_done + 8 * w, 0, t.watchdog, kWatchMma, abort);
+      }
     }
   } else {
     // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int w = warp >> 2, quad = warp & 3, r = quad * 32 + lane;  // row of the tile = TMEM lane
-    const uint32_t s_at = tmem + w * KT + (static_cast<uint32_t>(quad) << 21);
+    const uint32_t s_at0 = tmem + w * NB * KT + (static_cast<uint32_t>(quad) << 21);
     const uint32_t o_at = tmem + kO + w * DP + (static_cast<uint32_t>(quad) << 21);
     const float c = t.a.scale * kLog2e;
     const bool wide = t.wide != 0;
     float *bias_s = reinterpret_cast<float *>(base + L::kBias) + w * 2 * KT;
-    uint32_t seen = 0, done = 0, used = 0;
+    uint32_t seen = 0, used = 0;  // steps of this tile; slots passed
     bool ok = true;
     auto wait = [&](bool go, uint32_t bar, uint32_t parity) {
       const bool got = go && mbar_wait(bar, parity, t.watchdog, kWatchEpilogue, abort);
@@ -366,40 +409,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (r < KT) bias_s[(j & 1) * KT + r] = add;
           named_bar_sync(1 + w, 128);
         }
-        ok = wait(ok, s_full + 8 * w, seen++ & 1u);
+        const uint32_t buf = seen % NB, s_at = s_at0 + buf * KT;
+        ok = wait(ok, s_full + 16 * w + 8 * buf, seen / NB & 1u);
+        ++seen;
         if (!ok) continue;
-        // What takes no part becomes -inf; with a bias scores are in units of
-        // log2.  Four running maxima and sums: one of each would be a chain of
-        // 128 dependent operations.
         float2 s[KT / 32][16];
+        tmem_ld32(s_at, s[0]);
+        if (keys > 32) tmem_ld32(s_at + 32, s[1]);
+        tmem_ld_wait();
+        // What takes no part becomes -inf; with a bias the scores come in units of log2.
+        if (bias) {
+          const float4 *add = reinterpret_cast<const float4 *>(bias_s + (j & 1) * KT);
+#pragma unroll
+          for (int x = 0; x < KT / 2; x += 2) {
+            const float4 y = add[x / 2];
+            float2 &s0 = s[x / 16][x % 16], &s1 = s[x / 16][x % 16 + 1];
+            const float2 f0 = fma2(s0, make_float2(c, c), make_float2(y.x, y.y)), f1 = fma2(s1, make_float2(c, c), make_float2(y.z, y.w));
+            s0 = make_float2(y.x == -INFINITY ? -INFINITY : f0.x, y.y == -INFINITY ? -INFINITY : f0.y);
+            s1 = make_float2(y.z == -INFINITY ? -INFINITY : f1.x, y.w == -INFINITY ? -INFINITY : f1.y);
+          }
+        } else if (keys < KT) {
+#pragma unroll
+          for (int x = 0; x < KT / 2; ++x) {
+            float2 &s0 = s[x / 16][x % 16];
+            if (2 * x >= keys) s0.x = -INFINITY;
+            if (2 * x + 1 >= keys) s0.y = -INFINITY;
+          }
+        }
+        // Four running maxima and sums: one of each would be a chain of 64 dependent operations.
         float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c32 = 0; c32 < KT / 32; ++c32)
-          if (c32 * 32 < keys) tmem_ld32(s_at + c32 * 32, s[c32]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c32 = 0; c32 < KT / 32; ++c32) {
-          if (c32 * 32 >= keys) break;
-          if (bias) {
-            const float4 *add = reinterpret_cast<const float4 *>(bias_s + (j & 1) * KT + c32 * 32);
-#pragma unroll
-            for (int x = 0; x < 16; x += 2) {
-              const float4 y = add[x / 2];
-              const float2 f0 = fma2(s[c32][x], make_float2(c, c), make_float2(y.x, y.y));
-              const float2 f1 = fma2(s[c32][x + 1], make_float2(c, c), make_float2(y.z, y.w));
-              s[c32][x] = make_float2(y.x == -INFINITY ? -INFINITY : f0.x, y.y == -INFINITY ? -INFINITY : f0.y);
-              s[c32][x + 1] = make_float2(y.z == -INFINITY ? -INFINITY : f1.x, y.w == -INFINITY ? -INFINITY : f1.y);
-            }
-          } else if (c32 * 32 + 32 > keys) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              if (c32 * 32 + 2 * x >= keys) s[c32][x].x = -INFINITY;
-              if (c32 * 32 + 2 * x + 1 >= keys) s[c32][x].y = -INFINITY;
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[c32][x].x, s[c32][x].y));
-        }
+        for (int x = 0; x < KT / 2; ++x) most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[x / 16][x % 16].x, s[x / 16][x % 16].y));
         const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3])) * unit;
         const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
@@ -409,7 +449,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             sum *= keep;
           }
           if (j > 0) {
-            // the tensor core is done with O: S of this tile came after it
+            ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 2) % NB), (seen - 2) / NB & 1u);  // the step before's
+            if (!ok) continue;
 #pragma unroll 1
             for (int i = 0; i < dim; i += 32) {
               uint32_t o[32];
@@ -424,31 +465,33 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float from = top == -INFINITY ? 0.0f : top - kShift;
         float2 sum4[4] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-        for (int c32 = 0; c32 < KT / 32; ++c32) {
-          if (c32 * 32 >= keys) break;
-          uint32_t hi[16], lo[16];
+        for (int h = 0; h < KT / 32; ++h) {
+          if (32 * h >= keys) break;
+          uint32_t w32[32];  // 16 words high parts, 16 low
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            float2 p = fma2(s[c32][x], make_float2(unit, unit), make_float2(-from, -from));
+            float2 p = fma2(s[h][x], make_float2(unit, unit), make_float2(-from, -from));
             p = make_float2(ex2_approx(p.x), ex2_approx(p.y));
             sum4[x % 4] = add2(sum4[x % 4], p);
-            hi[x] = pack2<T>(p.x, p.y);
+            w32[x] = pack2<T>(p.x, p.y);
             if (kParts) {
-              const float2 back = unpack2<T>(hi[x]);
-              lo[x] = pack2<T>(p.x - back.x, p.y - back.y);
+              const float2 back = unpack2<T>(w32[x]);
+              w32[16 + x] = pack2<T>(p.x - back.x, p.y - back.y);
             }
           }
-          tmem_st16(s_at + c32 * 16, hi);
-          if (kParts) tmem_st16(s_at + KT / 2 + c32 * 16, lo);
+          if (kParts)
+            tmem_st32(s_at + 32 * h, w32);
+          else
+            tmem_st16(s_at + 32 * h, *reinterpret_cast<const uint32_t(*)[16]>(w32));
         }
         sum4[0] = add2(add2(sum4[0], sum4[1]), add2(sum4[2], sum4[3]));
         sum = sum4[0].x + sum4[0].y;
         tmem_st_wait();
         tc_fence_before();
         // Values of keys that take no part may be infinite or NaN, which a
-        // zero weight would not remove: tile 0's threads, one key each, clear
-        // them before the first product that reads them.
-        if (w == 0 && (bias || it.n < t.a.kv_len)) {
+        // zero weight would not remove: each tile's threads, one key each, clear
+        // them before its product reads them (both tiles write the same zeros).
+        if (bias || it.n < t.a.kv_len) {
           dead = dead && r < (keys + 15) / 16 * 16;
           if (__any_sync(0xffffffffu, dead)) {
             const uint32_t v_slot = (used + 1) % NS;
@@ -464,9 +507,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + 8 * w);
+        if (lane == 0) mbar_arrive(p_ready + 16 * w + 8 * buf);
       }
-      if (nt) ok = wait(ok, o_full + 8 * w, done++ & 1u);
+      if (nt) ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 1) % NB), (seen - 1) / NB & 1u);
       if (!ok) continue;
       const bool none = sum == 0.0f;  // then O is zero, or there was no tile
       const float inv = t.splits > 1 || none ? 1.0f : 1.0f / sum;
@@ -925,8 +968,8 @@ int run_attention(const struct htpg_attention_params *p, const AttnArgs &a, cons
     if (a.dim <= 128) return run_few<T, TO, 128>(p, a, d, st);
     return run_few<T, TO, 192>(p, a, d, st);
   }
-  if (a.dim <= 64) return run_tiles<T, TO, 64, 128>(p, a, d, st);
-  if (a.dim <= 128) return run_tiles<T, TO, 128, 128>(p, a, d, st);
+  if (a.dim <= 64) return run_tiles<T, TO, 64, 64>(p, a, d, st);
+  if (a.dim <= 128) return run_tiles<T, TO, 128, 64>(p, a, d, st);
   return run_tiles<T, TO, 192, 64>(p, a, d, st);
 }
 

@@ -377,22 +377,6 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Four of them over K = 64: the A columns advance by 8, the B descriptor by
-// b_step (in units of 16 bytes); one asm block, so nothing is scheduled between.
-__device__ __forceinline__ void umma_f16_ta4(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t b_step,
-                                             uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.eq.b32 q, %4, %4;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %6, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%7], %8, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%9], %10, %3, q;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_tmem + 8), "l"(b_desc + b_step), "r"(a_tmem + 16),
-      "l"(b_desc + 2 * b_step), "r"(a_tmem + 24), "l"(b_desc + 3 * b_step)
-      : "memory");
-}
 // Descriptor of an MN-major operand (K rows of 64 contiguous 16-bit M or N
 // elements, 128-byte swizzle): LBO is the distance of the next 64 elements, SBO
 // that of the next 8 K rows (1024 bytes).
