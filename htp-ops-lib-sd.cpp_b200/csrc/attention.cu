@@ -216,17 +216,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 9 && lane == 0) {
+    if (warp == 9) {
       // ------------------------------------------------------------ loads
       bool ok = true;
       uint32_t loads = 0, tiles[2] = {0, 0};  // K and V tiles, query tiles issued
       const int panels = (dim + 63) / 64;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, t.watchdog, kWatchProducer, abort)) != 0;
+      };
       auto load = [&](const CUtensorMap *map, int j, int h, int b) {
-        const uint32_t s = loads % NS, ph = loads / NS & 1u;
-        if (!mbar_wait(kv_empty + 8 * s, ph ^ 1u, t.watchdog, kWatchProducer, abort)) return false;
-        mbar_arrive_expect_tx(kv_full + 8 * s, panels * KT * 128);
-        for (int p = 0; p < panels; ++p)
-          tma_load_4d(kv_s + s * L::kStage + p * KT * 128, map, kv_full + 8 * s, p * 64, j * KT, h, b);
+        const uint32_t s = loads % NS, bar = kv_full + 8 * s;
+        if (!wait(kv_empty + 8 * s, (loads / NS & 1u) ^ 1u)) return false;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar, panels * KT * 128);
+          for (int p = 0; p < panels; ++p) tma_load_4d(kv_s + s * L::kStage + p * KT * 128, map, bar, p * 64, j * KT, h, b);
+        }
         ++loads;
         return true;
       };
@@ -234,12 +238,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const TileItem it = tile_item<KT>(t, item, lens);
         if (it.j0 == it.j1) continue;
         for (int w = 0; ok && w < (it.two ? 2 : 1); ++w) {
-          ok = mbar_wait(q_empty + 8 * w, (tiles[w] & 1u) ^ 1u, t.watchdog, kWatchProducer, abort);
+          ok = wait(q_empty + 8 * w, (tiles[w] & 1u) ^ 1u);
           if (!ok) break;
-          mbar_arrive_expect_tx(q_full + 8 * w, panels * 128 * 128);
-          for (int p = 0; p < panels; ++p)
-            tma_load_4d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, it.row0[w], it.head[w],
-                        it.b * t.q_batch);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(q_full + 8 * w, panels * 128 * 128);
+            for (int p = 0; p < panels; ++p)
+              tma_load_4d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, it.row0[w], it.head[w],
+                          it.b * t.q_batch);
+          }
           ++tiles[w];
           // the first keys right after the first tile's queries
           if (w == 0) ok = load(&map_k, it.j0, it.kvh * t.k_head, it.b * t.k_batch);
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp == 8 || warp == 10) {
       // ------------------------------------------------------------- MMAs
       // The whole warp runs the loop, so that descriptors stay in uniform
-      // registers; lane 0 issues.
+      // registers; one lane issues.
       const int w = warp == 10;
       const int ksteps = (dim + 15) / 16;
       const uint64_t desc_q = umma_desc_sw128(q_s + w * L::kQ), desc_k = umma_desc_sw128(kv_s);
@@ -309,10 +315,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           ok = ok && wait(kv_full + 8 * v_slot, v_phase);
           if (!ok) break;
           if (!old.mine) {
-            if (lane == 0) mbar_arrive(kv_empty + 8 * v_slot);
+            if (elect_one()) mbar_arrive(kv_empty + 8 * v_slot);
           } else {
             ++taken;
-            if (lane == 0) {
+            if (elect_one()) {
               // P of 32 keys (two K = 16 steps): 16 columns high parts, 16 low, where their scores were
               const uint64_t dv = desc_v + v_slot * (L::kStage / 16);
               const uint32_t p_t = s_t + buf * KT;
@@ -339,10 +345,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           ok = ok && wait(kv_full + 8 * k_slot, 2 * n / NS & 1u);
           if (!ok) break;
           if (!now.mine) {
-            if (lane == 0) mbar_arrive(kv_empty + 8 * k_slot);
+            if (elect_one()) mbar_arrive(kv_empty + 8 * k_slot);
           } else {
             const uint32_t buf = made++ % NB;
-            if (lane == 0) {
+            if (elect_one()) {
               uint64_t dq = desc_q, dk = desc_k + k_slot * (L::kStage / 16);
               const uint32_t idesc = kIdesc | (static_cast<uint32_t>((now.keys + 15) / 16 * 2) << 17);
               int i = 0;
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (NB > 1) past[0] = past[NB - 1];
         past[NB - 1] = now;
       }
-      if (lane == 0) {
+      if (elect_one()) {
         tc_commit(mma_done + 8 * w);  // every MMA is complete before TMEM is freed
         mbar_wait(mma_done + 8 * w, 0, t.watchdog, kWatchMma, abort);
       }

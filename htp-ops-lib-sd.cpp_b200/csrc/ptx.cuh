@@ -24,6 +24,20 @@ __device__ __forceinline__ uint64_t globaltimer() {
   return t;
 }
 
+// True in one lane of the (converged) warp, always the same one.  Unlike a
+// comparison of the lane number it tells the compiler that a single lane runs
+// the branch, so operands that instructions take from uniform registers
+// (descriptors, barriers) are moved there directly instead of lane by lane.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
