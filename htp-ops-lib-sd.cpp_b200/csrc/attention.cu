@@ -403,6 +403,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float *bias = t.a.bias ? t.a.bias + it.b * t.a.bias_stride : nullptr;
       const float unit = bias ? 1.0f : c;  // of the scores in s[], in log2
       float top = -INFINITY, sum = 0.0f;
+      if (w == 1 && nt) named_bar_arrive(3 + quad, 64);  // tile 0 begins
       for (int j = 0; j < nt; ++j, used += 2) {
         const int k0 = (it.j0 + j) * KT, keys = min(KT, it.n - k0);
         bool dead = r < KT && r >= keys;
@@ -418,80 +419,88 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t buf = seen % NB, s_at = s_at0 + buf * KT;
         ok = wait(ok, s_full + 16 * w + 8 * buf, seen / NB & 1u);
         ++seen;
-        if (!ok) continue;
         float2 s[KT / 32][16];
-        tmem_ld32(s_at, s[0]);
-        if (keys > 32) tmem_ld32(s_at + 32, s[1]);
-        tmem_ld_wait();
-        // What takes no part becomes -inf; with a bias the scores come in units of log2.
-        if (bias) {
-          const float4 *add = reinterpret_cast<const float4 *>(bias_s + (j & 1) * KT);
+        if (ok) {
+          tmem_ld32(s_at, s[0]);
+          if (keys > 32) tmem_ld32(s_at + 32, s[1]);
+          tmem_ld_wait();
+          // What takes no part becomes -inf; with a bias the scores come in units of log2.
+          if (bias) {
+            const float4 *add = reinterpret_cast<const float4 *>(bias_s + (j & 1) * KT);
 #pragma unroll
-          for (int x = 0; x < KT / 2; x += 2) {
-            const float4 y = add[x / 2];
-            float2 &s0 = s[x / 16][x % 16], &s1 = s[x / 16][x % 16 + 1];
-            const float2 f0 = fma2(s0, make_float2(c, c), make_float2(y.x, y.y)), f1 = fma2(s1, make_float2(c, c), make_float2(y.z, y.w));
-            s0 = make_float2(y.x == -INFINITY ? -INFINITY : f0.x, y.y == -INFINITY ? -INFINITY : f0.y);
-            s1 = make_float2(y.z == -INFINITY ? -INFINITY : f1.x, y.w == -INFINITY ? -INFINITY : f1.y);
-          }
-        } else if (keys < KT) {
+            for (int x = 0; x < KT / 2; x += 2) {
+              const float4 y = add[x / 2];
+              float2 &s0 = s[x / 16][x % 16], &s1 = s[x / 16][x % 16 + 1];
+              const float2 f0 = fma2(s0, make_float2(c, c), make_float2(y.x, y.y)), f1 = fma2(s1, make_float2(c, c), make_float2(y.z, y.w));
+              s0 = make_float2(y.x == -INFINITY ? -INFINITY : f0.x, y.y == -INFINITY ? -INFINITY : f0.y);
+              s1 = make_float2(y.z == -INFINITY ? -INFINITY : f1.x, y.w == -INFINITY ? -INFINITY : f1.y);
+            }
+          } else if (keys < KT) {
 #pragma unroll
-          for (int x = 0; x < KT / 2; ++x) {
-            float2 &s0 = s[x / 16][x % 16];
-            if (2 * x >= keys) s0.x = -INFINITY;
-            if (2 * x + 1 >= keys) s0.y = -INFINITY;
+            for (int x = 0; x < KT / 2; ++x) {
+              float2 &s0 = s[x / 16][x % 16];
+              if (2 * x >= keys) s0.x = -INFINITY;
+              if (2 * x + 1 >= keys) s0.y = -INFINITY;
+            }
           }
-        }
-        // Four running maxima and sums: one of each would be a chain of 64 dependent operations.
-        float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          // Four running maxima and sums: one of each would be a chain of 64 dependent operations.
+          float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < KT / 2; ++x) most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[x / 16][x % 16].x, s[x / 16][x % 16].y));
-        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3])) * unit;
-        const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
-        if (__any_sync(0xffffffffu, raise)) {
-          const float keep = raise ? ex2_approx(top - most) : 1.0f;
-          if (raise) {
-            top = most;
-            sum *= keep;
-          }
-          if (j > 0) {
-            ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 2) % NB), (seen - 2) / NB & 1u);  // the step before's
-            if (!ok) continue;
+          for (int x = 0; x < KT / 2; ++x) most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[x / 16][x % 16].x, s[x / 16][x % 16].y));
+          const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3])) * unit;
+          const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
+          if (__any_sync(0xffffffffu, raise)) {
+            const float keep = raise ? ex2_approx(top - most) : 1.0f;
+            if (raise) {
+              top = most;
+              sum *= keep;
+            }
+            if (j > 0) {
+              ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 2) % NB), (seen - 2) / NB & 1u);  // the step before's
 #pragma unroll 1
-            for (int i = 0; i < dim; i += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_at + i, o);
-              tmem_ld_wait();
+              for (int i = 0; ok && i < dim; i += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_at + i, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
-              tmem_st32(o_at + i, o);
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                tmem_st32(o_at + i, o);
+              }
             }
           }
         }
-        const float from = top == -INFINITY ? 0.0f : top - kShift;
-        float2 sum4[4] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        // The two tiles' warps of one scheduler take turns at the exponentials, so
+        // that one's run while the other waits, loads and compares (left alone
+        // they fall into step, and the exponential unit idles in between).
+        if (it.two) named_bar_sync(3 + 4 * w + quad, 64);
+        if (ok) {
+          const float from = top == -INFINITY ? 0.0f : top - kShift;
+          float2 sum4[4] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-        for (int h = 0; h < KT / 32; ++h) {
-          if (32 * h >= keys) break;
-          uint32_t w32[32];  // 16 words high parts, 16 low
+          for (int h = 0; h < KT / 32; ++h) {
+            if (32 * h >= keys) break;
+            uint32_t w32[32];  // 16 words high parts, 16 low
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            float2 p = fma2(s[h][x], make_float2(unit, unit), make_float2(-from, -from));
-            p = make_float2(ex2_approx(p.x), ex2_approx(p.y));
-            sum4[x % 4] = add2(sum4[x % 4], p);
-            w32[x] = pack2<T>(p.x, p.y);
-            if (kParts) {
-              const float2 back = unpack2<T>(w32[x]);
-              w32[16 + x] = pack2<T>(p.x - back.x, p.y - back.y);
+            for (int x = 0; x < 16; ++x) {
+              float2 p = fma2(s[h][x], make_float2(unit, unit), make_float2(-from, -from));
+              p = make_float2(ex2_approx(p.x), ex2_approx(p.y));
+              sum4[x % 4] = add2(sum4[x % 4], p);
+              w32[x] = pack2<T>(p.x, p.y);
+              if (kParts) {
+                const float2 back = unpack2<T>(w32[x]);
+                w32[16 + x] = pack2<T>(p.x - back.x, p.y - back.y);
+              }
             }
+            if (kParts)
+              tmem_st32(s_at + 32 * h, w32);
+            else
+              tmem_st16(s_at + 32 * h, *reinterpret_cast<const uint32_t(*)[16]>(w32));
           }
-          if (kParts)
-            tmem_st32(s_at + 32 * h, w32);
-          else
-            tmem_st16(s_at + 32 * h, *reinterpret_cast<const uint32_t(*)[16]>(w32));
+          sum4[0] = add2(add2(sum4[0], sum4[1]), add2(sum4[2], sum4[3]));
+          sum = sum4[0].x + sum4[0].y;
         }
-        sum4[0] = add2(add2(sum4[0], sum4[1]), add2(sum4[2], sum4[3]));
-        sum = sum4[0].x + sum4[0].y;
+        if (it.two && (w == 0 || j + 1 < nt)) named_bar_arrive(3 + 4 * (1 - w) + quad, 64);
+        if (!ok) continue;
         tmem_st_wait();
         tc_fence_before();
         // Values of keys that take no part may be infinite or NaN, which a
