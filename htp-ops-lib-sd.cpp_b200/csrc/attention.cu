@@ -54,13 +54,14 @@ struct TileArgs {
   int row_tiles;       // 128-row tiles of one head
   int pairs;           // tile pairs of one key/value head: ceil(group * row_tiles / 2)
   int kv_heads;
-  int splits;          // ranges of keys of one pair
-  int items;           // batch * kv_heads * pairs * splits
+  int units;           // batch * kv_heads * pairs
+  int whole;           // the first units are one item each,
+  int splits;          // the others this many: ranges of their keys
+  int items;           // whole + (units - whole) * splits
   int q_batch, k_batch, k_head, v_batch, v_head;  // 0: that dimension's stride is 0 (one copy)
   int wide;            // output rows are 32-byte aligned
-  float *part_o;       // splits > 1: [splits][rows][dim] sums
-  float2 *part_ml;     //             [splits][rows] maximum (log2) and sum
-  long long rows;
+  float *part_o;       // of split items: [item - whole][tile][128 rows][dim] sums
+  float2 *part_ml;     // [item - whole][tile][128 rows] maximum (log2) and sum
   uint32_t *watchdog;
 };
 
@@ -91,10 +92,13 @@ template <int KT>
 __device__ __forceinline__ TileItem tile_item(const TileArgs &t, int item, const int *lens) {
   TileItem r;
   uint32_t u = item, pair;
+  int splits = 1;
   r.split = 0;
-  if (t.splits > 1) {
-    u = u / t.splits;
-    r.split = item - u * t.splits;
+  if (item >= t.whole) {
+    splits = t.splits;
+    u = (item - t.whole) / splits;
+    r.split = item - t.whole - u * splits;
+    u += t.whole;
   }
   pair = u;
   u = u / t.pairs;
@@ -102,7 +106,7 @@ __device__ __forceinline__ TileItem tile_item(const TileArgs &t, int item, const
   r.b = u / t.kv_heads;
   r.kvh = u - r.b * t.kv_heads;
   r.n = r.b < kLensHeld ? lens[r.b] : clamped_len(t.a, r.b);
-  const int tiles = (r.n + KT - 1) / KT, per = (tiles + t.splits - 1) / t.splits;
+  const int tiles = (r.n + KT - 1) / KT, per = (tiles + splits - 1) / splits;
   r.j0 = min(r.split * per, tiles);
   r.j1 = min(r.j0 + per, tiles);
   r.two = 2 * static_cast<int>(pair) + 1 < t.a.group * t.row_tiles;
@@ -527,11 +531,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (nt) ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 1) % NB), (seen - 1) / NB & 1u);
       if (!ok) continue;
       const bool none = sum == 0.0f;  // then O is zero, or there was no tile
-      const float inv = t.splits > 1 || none ? 1.0f : 1.0f / sum;
-      const long long row = (static_cast<long long>(it.b) * t.a.q_heads + it.head[w]) * t.a.q_len + it.row0[w] + r;
+      const bool split = item >= t.whole;
+      const float inv = split || none ? 1.0f : 1.0f / sum;
+      const long long row = (static_cast<long long>(item - t.whole) * 2 + w) * 128 + r;  // of the parts
       TO *out = static_cast<TO *>(t.a.out) + it.b * t.a.os[0] + static_cast<long long>(it.row0[w] + r) * t.a.os[1] +
                 it.head[w] * t.a.os[2];
-      float *part = t.splits > 1 ? t.part_o + (it.split * t.rows + row) * dim : nullptr;
+      float *part = split ? t.part_o + row * dim : nullptr;
 #pragma unroll 1
       for (int i = 0; i < dim; i += 32) {
         float o[32];
@@ -548,7 +553,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             store_columns<TO>(out, i, dim, o, wide);
         }
       }
-      if (part && mine) t.part_ml[it.split * t.rows + row] = make_float2(none ? -INFINITY : top, sum);
+      if (part && mine) t.part_ml[row] = make_float2(none ? -INFINITY : top, sum);
       tc_fence_before();  // O has been read before the next tile's P is announced
     }
   }
@@ -561,31 +566,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
-// Joins the key ranges of each row in order: one warp per row.
+// Joins the key ranges of the split units' rows, in order: one warp per row.
 template <typename TO>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ TileArgs t) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= t.rows) return;
+  const int index = blockIdx.x * 8 + (threadIdx.x >> 5);  // unit, tile, row
+  const int unit = index / 256, w = index / 128 % 2, r = index % 128;
+  const uint32_t u = t.whole + unit, pair = u % t.pairs, tile = 2 * pair + w;
+  const int kvh = u / t.pairs % t.kv_heads, b = u / t.pairs / t.kv_heads;
+  if (tile >= static_cast<uint32_t>(t.a.group) * t.row_tiles) return;
+  const int i = tile % t.row_tiles * 128 + r, h = kvh * t.a.group + tile / t.row_tiles;
+  if (i >= t.a.q_len) return;
+  const long long first = (static_cast<long long>(unit) * t.splits * 2 + w) * 128 + r;  // the ranges: 256 rows apart
   float top = -INFINITY;
-  for (int s = 0; s < t.splits; ++s) top = fmaxf(top, t.part_ml[s * t.rows + row].x);
+  for (int s = 0; s < t.splits; ++s) top = fmaxf(top, t.part_ml[first + s * 256].x);
   const float from = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
   for (int s = 0; s < t.splits; ++s) {
-    const float2 ml = t.part_ml[s * t.rows + row];
+    const float2 ml = t.part_ml[first + s * 256];
     sum += ml.y * ex2_approx(ml.x - from);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const long long i = row % t.a.q_len, h = row / t.a.q_len % t.a.q_heads, b = row / t.a.q_len / t.a.q_heads;
   TO *out = static_cast<TO *>(t.a.out) + b * t.a.os[0] + i * t.a.os[1] + h * t.a.os[2];
   for (int d = lane; d < t.a.dim; d += 32) {
     float o = 0.0f;
     for (int s = 0; s < t.splits; ++s)
-      o += t.part_o[(s * t.rows + row) * t.a.dim + d] * ex2_approx(t.part_ml[s * t.rows + row].x - from);
+      o += t.part_o[(first + s * 256) * t.a.dim + d] * ex2_approx(t.part_ml[first + s * 256].x - from);
     out[d] = from_f32<TO>(sum == 0.0f ? 0.0f : o * inv);
   }
 }
+
 // ------------------------------------------------------------ few rows
 // Up to 16 query rows that share one key/value head (the tokens of a decode
 // step times the heads of a group): bound by reading K and V once.  Four warps
@@ -878,14 +889,20 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   const long long pairs = (static_cast<long long>(a.group) * t.row_tiles + 1) / 2;
   if (pairs > 0x3fffffff) return HTPG_ECAPACITY;
   t.pairs = static_cast<int>(pairs);
-  t.rows = static_cast<long long>(a.batch) * a.q_heads * a.q_len;
   t.watchdog = d.watchdog;
   const long long units = pairs * t.kv_heads * a.batch;
   const int tiles = (a.kv_len + KT - 1) / KT;
-  t.splits = 1;
-  if (units * 2 <= d.sms && tiles >= 4) t.splits = static_cast<int>(std::min<long long>(d.sms / units, tiles / 2));
-  if (units * t.splits > 0x3fffffff) return HTPG_ECAPACITY;
-  t.items = static_cast<int>(units * t.splits);
+  if (units * 64 > 0x3fffffff) return HTPG_ECAPACITY;
+  // Rounds of one unit per SM; the units of a last round that would leave half
+  // of the SMs idle or more are cut into ranges of keys, where a range of two tiles
+  // or more per part is left and the round gets shorter by more than the joining (4 tiles or so).
+  const int rest = static_cast<int>(units % d.sms);
+  int splits = rest ? std::min(d.sms / rest, tiles / 2) : 1;
+  if (splits < 2 || tiles - (tiles + splits - 1) / splits < 4) splits = 1;
+  t.units = static_cast<int>(units);
+  t.whole = splits > 1 ? t.units - rest : t.units;
+  t.splits = splits;
+  t.items = t.whole + (t.units - t.whole) * splits;
   t.wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
   const int qe[3] = {a.batch, a.q_len, a.q_heads};
   for (int i = 0; i < 3; ++i)
@@ -902,8 +919,8 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
     lock = op_lock();
     uint32_t *counters;
     uint8_t *scratch;
-    const size_t ml = (static_cast<size_t>(t.splits) * t.rows * sizeof(float2) + 255) / 256 * 256;
-    rc = op_scratch(st, ml + static_cast<size_t>(t.splits) * t.rows * a.dim * 4, &counters, &scratch);
+    const size_t rows = static_cast<size_t>(t.items - t.whole) * 256, ml = rows * sizeof(float2);
+    rc = op_scratch(st, ml + rows * a.dim * 4, &counters, &scratch);
     if (rc) return rc;
     t.part_ml = reinterpret_cast<float2 *>(scratch);
     t.part_o = reinterpret_cast<float *>(scratch + ml);
@@ -915,7 +932,7 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   e = op_launch(fn, dim3(static_cast<unsigned>(std::min(t.items, d.sms))), kTileThreads, L::kBytes, st, mq, mk,
                 mv, t);
   if (e == cudaSuccess && t.splits > 1)
-    e = op_launch(attn_join_kernel<TO>, dim3(static_cast<unsigned>((t.rows + 7) / 8)), 256, 0, st, t);
+    e = op_launch(attn_join_kernel<TO>, dim3((t.units - t.whole) * 32), 256, 0, st, t);
   return op_result(e);
 }
 
