@@ -51,14 +51,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct TileArgs {
   AttnArgs a;
-  int row_tiles;       // 128-row tiles of one head
-  int pairs;           // tile pairs of one key/value head: ceil(group * row_tiles / 2)
+  int pack;            // heads of a group that share a tile (rows token by token), a power of two, or 1
+  int row_tiles;       // tiles of one head, or of one group's heads together
+  int tiles;           // tiles of one key/value head
+  int pairs;           // tile pairs of one key/value head
   int kv_heads;
   int units;           // batch * kv_heads * pairs
   int whole;           // the first units are one item each,
   int splits;          // the others this many: ranges of their keys
   int items;           // whole + (units - whole) * splits
-  int q_batch, k_batch, k_head, v_batch, v_head;  // 0: that dimension's stride is 0 (one copy)
+  int q_batch, q_head, k_batch, k_head, v_batch, v_head;  // 0: that dimension's stride is 0 (one copy)
   int wide;            // output rows are 32-byte aligned
   float *part_o;       // of split items: [item - whole][tile][128 rows][dim] sums
   float2 *part_ml;     // [item - whole][tile][128 rows] maximum (log2) and sum
@@ -80,7 +82,7 @@ struct TileSmem {
 
 struct TileItem {
   int b, kvh, n, j0, j1, split;  // n keys take part, tiles [j0, j1) of them are this item's
-  int head[2], row0[2];
+  int head[2], row0[2];  // first head and token of each tile
   bool two;
 };
 
@@ -109,12 +111,12 @@ __device__ __forceinline__ TileItem tile_item(const TileArgs &t, int item, const
   const int tiles = (r.n + KT - 1) / KT, per = (tiles + splits - 1) / splits;
   r.j0 = min(r.split * per, tiles);
   r.j1 = min(r.j0 + per, tiles);
-  r.two = 2 * static_cast<int>(pair) + 1 < t.a.group * t.row_tiles;
+  r.two = 2 * static_cast<int>(pair) + 1 < t.tiles;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const uint32_t tile = 2 * pair + w, head = t.a.group == 1 ? 0 : tile / t.row_tiles;
+    const uint32_t tile = 2 * pair + w, head = t.tiles == t.row_tiles ? 0 : tile / t.row_tiles;
     r.head[w] = r.kvh * t.a.group + head;
-    r.row0[w] = (tile - head * t.row_tiles) * 128;
+    r.row0[w] = (tile - head * t.row_tiles) * (128 / t.pack);
   }
   return r;
 }
@@ -247,8 +249,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (elect_one()) {
             mbar_arrive_expect_tx(q_full + 8 * w, panels * 128 * 128);
             for (int p = 0; p < panels; ++p)
-              tma_load_4d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, it.row0[w], it.head[w],
-                          it.b * t.q_batch);
+              tma_load_5d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, 0, it.row0[w],
+                          (t.pack > 1 ? it.kvh : it.head[w]) * t.q_head, it.b * t.q_batch);
           }
           ++tiles[w];
           // the first keys right after the first tile's queries
@@ -403,7 +405,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         used += 2 * nt;
         continue;
       }
-      const bool mine = it.row0[w] + r < t.a.q_len;
+      const int token = it.row0[w] + r / t.pack, head = it.head[w] + r % t.pack;
+      const bool mine = token < t.a.q_len;
       const float *bias = t.a.bias ? t.a.bias + it.b * t.a.bias_stride : nullptr;
       const float unit = bias ? 1.0f : c;  // of the scores in s[], in log2
       float top = -INFINITY, sum = 0.0f;
@@ -534,8 +537,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool split = item >= t.whole;
       const float inv = split || none ? 1.0f : 1.0f / sum;
       const long long row = (static_cast<long long>(item - t.whole) * 2 + w) * 128 + r;  // of the parts
-      TO *out = static_cast<TO *>(t.a.out) + it.b * t.a.os[0] + static_cast<long long>(it.row0[w] + r) * t.a.os[1] +
-                it.head[w] * t.a.os[2];
+      TO *out = static_cast<TO *>(t.a.out) + it.b * t.a.os[0] + token * t.a.os[1] + head * t.a.os[2];
       float *part = split ? t.part_o + row * dim : nullptr;
 #pragma unroll 1
       for (int i = 0; i < dim; i += 32) {
@@ -575,8 +577,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
   const int unit = index / 256, w = index / 128 % 2, r = index % 128;
   const uint32_t u = t.whole + unit, pair = u % t.pairs, tile = 2 * pair + w;
   const int kvh = u / t.pairs % t.kv_heads, b = u / t.pairs / t.kv_heads;
-  if (tile >= static_cast<uint32_t>(t.a.group) * t.row_tiles) return;
-  const int i = tile % t.row_tiles * 128 + r, h = kvh * t.a.group + tile / t.row_tiles;
+  if (tile >= static_cast<uint32_t>(t.tiles)) return;
+  const int i = tile % t.row_tiles * (128 / t.pack) + r / t.pack;
+  const int h = kvh * t.a.group + tile / t.row_tiles + r % t.pack;
   if (i >= t.a.q_len) return;
   const long long first = (static_cast<long long>(unit) * t.splits * 2 + w) * 128 + r;  // the ranges: 256 rows apart
   float top = -INFINITY;
@@ -863,42 +866,64 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
   if (threadIdx.x == 0) f.counters[unit] = 0;
 }
 
-// A 4-D map {dim, tokens, heads, batch} of one operand, boxes of 64 x box_rows.
-// Heads or batches that share one copy (stride 0) become one; strides of
-// extents of one are not looked at.
-int operand_map(CUtensorMap *map, int type, const void *base, int dim, int tokens, int heads, int batch,
-                const int64_t *stride, int box_rows, int *head_step, int *batch_step) {
-  *head_step = heads > 1 && stride[2] != 0;
-  *batch_step = batch > 1 && stride[0] != 0;
-  const uint64_t row = static_cast<uint64_t>(dim) * 2;
-  const uint64_t dims[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(tokens),
-                            static_cast<uint64_t>(*head_step ? heads : 1), static_cast<uint64_t>(*batch_step ? batch : 1)};
-  const uint64_t strides[3] = {tokens > 1 ? static_cast<uint64_t>(stride[1]) * 2 : row,
-                               *head_step ? static_cast<uint64_t>(stride[2]) * 2 : row,
-                               *batch_step ? static_cast<uint64_t>(stride[0]) * 2 : row};
+// Stride (bytes) of an extent: its own where it is stepped along, any valid one otherwise.
+uint64_t step_of(bool stepped, int64_t stride, int dim) { return static_cast<uint64_t>(stepped ? stride : dim) * 2; }
+
+// A map {dim, tokens, heads, batch} of K or V, boxes of 64 x box_rows.  Heads or
+// batches that share one copy (stride 0) become one.
+int kv_map(CUtensorMap *map, const struct htpg_attention_params *p, const void *base, const int64_t *stride, int box_rows,
+           int *head_step, int *batch_step) {
+  *head_step = p->kv_heads > 1 && stride[2] != 0;
+  *batch_step = p->batch > 1 && stride[0] != 0;
+  const uint64_t dims[4] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(p->kv_len),
+                            static_cast<uint64_t>(*head_step ? p->kv_heads : 1), static_cast<uint64_t>(*batch_step ? p->batch : 1)};
+  const uint64_t strides[3] = {step_of(p->kv_len > 1, stride[1], p->head_dim), step_of(*head_step, stride[2], p->head_dim),
+                               step_of(*batch_step, stride[0], p->head_dim)};
   const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
-  return op_tensor_map(map, type, base, dims, strides, box);
+  return op_tensor_map(map, p->type, base, 4, dims, strides, box);
+}
+
+// A map {dim, packed heads, tokens, heads or groups, batch} of Q, boxes of 128
+// rows: 128 / pack tokens, each with `pack` heads.
+int q_map(CUtensorMap *map, const struct htpg_attention_params *p, const void *base, int pack, int *head_step,
+          int *batch_step) {
+  const int64_t *stride = p->q_stride;
+  *head_step = p->q_heads > pack && stride[2] != 0;
+  const int others = *head_step ? p->q_heads / pack : 1;
+  *batch_step = p->batch > 1 && stride[0] != 0;
+  const uint64_t dims[5] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(pack), static_cast<uint64_t>(p->q_len),
+                            static_cast<uint64_t>(others), static_cast<uint64_t>(*batch_step ? p->batch : 1)};
+  const uint64_t strides[4] = {step_of(pack > 1, stride[2], p->head_dim), step_of(p->q_len > 1, stride[1], p->head_dim),
+                               step_of(others > 1, stride[2] * pack, p->head_dim), step_of(*batch_step, stride[0], p->head_dim)};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(pack), static_cast<uint32_t>(128 / pack), 1, 1};
+  return op_tensor_map(map, p->type, base, 5, dims, strides, box);
 }
 
 template <typename T, typename TO, int DP, int KT>
 int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const OpDevice &d, cudaStream_t st) {
   TileArgs t = {};
   t.a = a;
-  t.row_tiles = (a.q_len + 127) / 128;
+  // A group's heads share tiles where their number divides 128: few tokens then
+  // fill a tile (16 tokens x 4 heads in one tile instead of four).
+  t.pack = (a.group & (a.group - 1)) == 0 && a.group <= 128 && p->q_stride[2] != 0 ? a.group : 1;
   t.kv_heads = p->kv_heads;
-  const long long pairs = (static_cast<long long>(a.group) * t.row_tiles + 1) / 2;
-  if (pairs > 0x3fffffff) return HTPG_ECAPACITY;
+  const long long row_tiles = (static_cast<long long>(a.q_len) * t.pack + 127) / 128, tiles_kv = row_tiles * (a.group / t.pack);
+  const long long pairs = (tiles_kv + 1) / 2;
+  if (pairs > 0x3ffffff) return HTPG_ECAPACITY;
+  t.row_tiles = static_cast<int>(row_tiles);
+  t.tiles = static_cast<int>(tiles_kv);
   t.pairs = static_cast<int>(pairs);
   t.watchdog = d.watchdog;
   const long long units = pairs * t.kv_heads * a.batch;
   const int tiles = (a.kv_len + KT - 1) / KT;
   if (units * 64 > 0x3fffffff) return HTPG_ECAPACITY;
   // Rounds of one unit per SM; the units of a last round that would leave half
-  // of the SMs idle or more are cut into ranges of keys, where a range of two tiles
-  // or more per part is left and the round gets shorter by more than the joining (4 tiles or so).
+  // of the SMs idle or more are cut into ranges of keys of two tiles or
+  // more, where the round gets shorter by 12 tiles (8 tiles cut in four: 84 -> 88 us
+  // in all; 64 cut in five: 455 -> 416).
   const int rest = static_cast<int>(units % d.sms);
   int splits = rest ? std::min(d.sms / rest, tiles / 2) : 1;
-  if (splits < 2 || tiles - (tiles + splits - 1) / splits < 4) splits = 1;
+  if (splits < 2 || tiles - (tiles + splits - 1) / splits < 12) splits = 1;
   t.units = static_cast<int>(units);
   t.whole = splits > 1 ? t.units - rest : t.units;
   t.splits = splits;
@@ -908,11 +933,9 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   for (int i = 0; i < 3; ++i)
     if (qe[i] > 1 && a.os[i] * sizeof(TO) % 32) t.wide = 0;
   CUtensorMap mq, mk, mv;
-  int q_head, rc;
-  // a query head or token stride of 0 needs no map of its own: refused by the caller
-  if ((rc = operand_map(&mq, p->type, a.q, a.dim, a.q_len, a.q_heads, a.batch, p->q_stride, 128, &q_head, &t.q_batch)) ||
-      (rc = operand_map(&mk, p->type, a.k, a.dim, a.kv_len, p->kv_heads, a.batch, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
-      (rc = operand_map(&mv, p->type, a.v, a.dim, a.kv_len, p->kv_heads, a.batch, p->v_stride, KT, &t.v_head, &t.v_batch)))
+  int rc;
+  if ((rc = q_map(&mq, p, a.q, t.pack, &t.q_head, &t.q_batch)) || (rc = kv_map(&mk, p, a.k, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
+      (rc = kv_map(&mv, p, a.v, p->v_stride, KT, &t.v_head, &t.v_batch)))
     return rc;
   std::unique_lock<std::mutex> lock;
   if (t.splits > 1) {

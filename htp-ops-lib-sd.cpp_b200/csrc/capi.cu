@@ -1170,16 +1170,16 @@ int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scr
   return HTPG_OK;
 }
 
-int op_tensor_map(CUtensorMap *map, int type, const void *base, const uint64_t (&dims)[4],
-                  const uint64_t (&strides)[3], const uint32_t (&box)[4]) {
-  if (!g_encode) return HTPG_ELAUNCH;
-  cuuint64_t d[4], s[3];
-  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
-  for (int i = 0; i < 4; ++i) d[i] = dims[i], b[i] = box[i];
-  for (int i = 0; i < 3; ++i) s[i] = strides[i];
+int op_tensor_map(CUtensorMap *map, int type, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
+                  const uint32_t *box) {
+  if (!g_encode || rank < 2 || rank > 5) return HTPG_ELAUNCH;
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
+  for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
   const CUresult r = g_encode(map,
                               type == HTPG_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                              4, const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              rank, const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {

@@ -36,10 +36,10 @@ std::unique_lock<std::mutex> op_lock();
 // captured graph may refer to is never freed.
 constexpr int kOpCounters = 16384;
 int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch);
-// Tensor map of a 16-bit array of up to 4 dimensions (innermost first; strides
-// in bytes of dimensions 1 .. 3), zero fill, 128-byte swizzle.
-int op_tensor_map(CUtensorMap *map, int type, const void *base, const uint64_t (&dims)[4],
-                  const uint64_t (&strides)[3], const uint32_t (&box)[4]);
+// Tensor map of a 16-bit array of `rank` <= 5 dimensions (innermost first;
+// strides in bytes of dimensions 1 .. rank - 1), zero fill, 128-byte swizzle.
+int op_tensor_map(CUtensorMap *map, int type, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
+                  const uint32_t *box);
 
 // Launch as a programmatic dependent: the kernel waits (grid_dependency_wait)
 // before it touches memory, so only its set-up overlaps the kernel before it.

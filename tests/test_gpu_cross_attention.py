@@ -91,6 +91,7 @@ TYPES = [(F16, F32), (F16, F16), (BF16, BF16), (BF16, F32)]
     (2, 17, 2, 3, 3, 72), (2, 127, 128, 4, 4, 64), (1, 128, 129, 4, 2, 128), (2, 129, 127, 2, 1, 96),
     (1, 256, 257, 3, 3, 40), (2, 300, 640, 2, 2, 192), (1, 513, 1000, 2, 1, 8), (1, 1000, 77, 5, 5, 64),
     (1, 65, 2500, 2, 2, 128), (3, 40, 5000, 1, 1, 64), (1, 2000, 16, 1, 1, 128),
+    (2, 16, 300, 32, 8, 128), (1, 5, 200, 128, 1, 64), (1, 33, 150, 24, 3, 64), (1, 9, 100, 12, 2, 40), (1, 2, 70, 256, 1, 64),
 ])
 def test_matches_fp64(gpu, b, n, m, h, hk, d, src, dst):
     q, k, v, _ = inputs(gpu, b, n, m, h, hk, d, src)
@@ -184,6 +185,10 @@ def test_layouts(gpu, n):
     bias = torch.randn(1, m, generator=g, device=gpu)
     out, _ = call(q, k1, v1, F16, bias=bias, bias_stride=0)
     close(out, q, k1, v1, scale, None, bias.expand(b, -1))
+    # one copy of the queries for every head, and for every batch
+    for qe in (q[:, :, :1].expand(-1, -1, h, -1), q[:1].expand(b, -1, -1, -1)):
+        out, _ = call(qe, k, v, F16)
+        close(out, qe, k, v, scale)
     # one batch, one head, strides of extents of one are not looked at
     q1 = q[:1, :, :1].as_strided((1, n, 1, d), (3, q.stride(1), 5, 1))
     k2 = k[:1, :, :1].as_strided((1, m, 1, d), (1, k.stride(1), 7, 1))
