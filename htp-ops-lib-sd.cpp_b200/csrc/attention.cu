@@ -61,24 +61,34 @@ struct TileArgs {
   int splits;          // the others this many: ranges of their keys
   int items;           // whole + (units - whole) * splits
   int q_batch, q_head, k_batch, k_head, v_batch, v_head;  // 0: that dimension's stride is 0 (one copy)
+  int staged;          // the output has a tensor map (boxes of one warp's 32 rows)
   int wide;            // output rows are 32-byte aligned
   float *part_o;       // of split items: [item - whole][tile][128 rows][dim] sums
   float2 *part_ml;     // [item - whole][tile][128 rows] maximum (log2) and sum
   uint32_t *watchdog;
 };
 
-template <int DP, int KT>
+// STAGED: output rows leave through shared memory (FP32 rows of up to 128: twice
+// the stores of 16-bit ones, which gain nothing: 2 x 4096 rows of 64 over 77 keys
+// 32.7 -> 29.4 us with FP32 outputs, 28.6 -> 30.4 with FP16).
+template <int DP, int KT, bool STAGED>
 struct TileSmem {
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kStage = KT * DP * 2;
-  static constexpr int kStages = DP == 128 ? 8 : DP == 64 ? 10 : 5;
+  static constexpr int kStages = DP == 128 ? (STAGED ? 7 : 8) : DP == 64 ? 10 : 5;
   static constexpr int kBuffers = DP == 192 ? 1 : 2;  // of S, per tile
   static constexpr int kBarriers = 2 * kStages + 18;
-  static constexpr int kBars = 2 * kQ + kStages * kStage;
+  static constexpr int kOut = 2 * kQ + kStages * kStage;
+  static constexpr int kBars = kOut + (STAGED ? 8 * 4096 : 0);  // 4 KB per softmax warp
   static constexpr int kLens = kBars + 8 * kBarriers + 24;
   static constexpr int kBias = (kLens + 4 * kLensHeld + 15) / 16 * 16;  // [tile][2][KT]
   static constexpr int kBytes = kBias + 16 * KT + 1024;                 // + alignment
 };
+
+template <typename TO>
+constexpr bool tile_staged(int dp) {
+  return sizeof(TO) == 4 && dp <= 128;
+}
 
 struct TileItem {
   int b, kvh, n, j0, j1, split;  // n keys take part, tiles [j0, j1) of them are this item's
@@ -162,8 +172,10 @@ __device__ __forceinline__ void store_columns(TO *row, int c, int dim, const flo
 template <typename T, typename TO, int DP, int KT>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attn_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TileArgs t) {
-  using L = TileSmem<DP, KT>;
+                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+                     const __grid_constant__ TileArgs t) {
+  constexpr bool kStaged = tile_staged<TO>(DP);
+  using L = TileSmem<DP, KT, kStaged>;
   // FP32 outputs: P in two 16-bit parts, high and low, each KT / 2 TMEM columns
   constexpr bool kParts = sizeof(TO) == 4;
   // FP16 weights are 2^7 times larger, so that those below 2^-14 of the
@@ -539,26 +551,57 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const long long row = (static_cast<long long>(item - t.whole) * 2 + w) * 128 + r;  // of the parts
       TO *out = static_cast<TO *>(t.a.out) + it.b * t.a.os[0] + token * t.a.os[1] + head * t.a.os[2];
       float *part = split ? t.part_o + row * dim : nullptr;
+      if (kStaged && t.staged && !split) {
+        // Rows of one thread become 128-byte pieces of 32 rows, stored by TMA
+        // (which leaves out rows and columns past the ends): straight from the
+        // threads, every store would touch 32 lines.
+        const uint32_t stage = q_s + L::kOut + warp * 4096, at = stage + lane * 128;
+        const int first = it.row0[w] + quad * 32 / t.pack;
 #pragma unroll 1
-      for (int i = 0; i < dim; i += 32) {
-        float o[32];
-        if (nt) {
-          tmem_ld32(o_at + i, o);
-          tmem_ld_wait();
-        }
+        for (int i = 0; i < dim; i += 32) {
+          float o[32];
+          if (nt) {
+            tmem_ld32(o_at + i, o);
+            tmem_ld_wait();
+          }
+          uint32_t words[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) o[x] = nt ? o[x] * inv : 0.0f;
-        if (mine) {
-          if (part)
-            store_columns<float>(part, i, dim, o, true);
-          else
-            store_columns<TO>(out, i, dim, o, wide);
+          for (int x = 0; x < 32; ++x) words[x] = nt ? __float_as_uint(o[x] * inv) : 0u;
+          if (elect_one()) bulk_wait_read_all();  // the piece before has left
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            sts_u32x4(at + ((x ^ (lane & 7)) << 4), words[4 * x], words[4 * x + 1], words[4 * x + 2], words[4 * x + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (first < t.a.q_len && elect_one()) {
+            tma_store_5d(&map_out, stage, i, 0, first, t.pack > 1 ? it.kvh : it.head[w], it.b);
+            bulk_commit();
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < dim; i += 32) {
+          float o[32];
+          if (nt) {
+            tmem_ld32(o_at + i, o);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = nt ? o[x] * inv : 0.0f;
+          if (mine) {
+            if (part)
+              store_columns<float>(part, i, dim, o, true);
+            else
+              store_columns<TO>(out, i, dim, o, wide);
+          }
         }
       }
       if (part && mine) t.part_ml[row] = make_float2(none ? -INFINITY : top, sum);
       tc_fence_before();  // O has been read before the next tile's P is announced
     }
   }
+  if (kStaged && warp < 8 && elect_one()) bulk_wait_all();  // output pieces still leaving
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
@@ -867,7 +910,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
 }
 
 // Stride (bytes) of an extent: its own where it is stepped along, any valid one otherwise.
-uint64_t step_of(bool stepped, int64_t stride, int dim) { return static_cast<uint64_t>(stepped ? stride : dim) * 2; }
+uint64_t step_of(bool stepped, int64_t stride, int dim, int bytes) { return static_cast<uint64_t>(stepped ? stride : dim) * bytes; }
 
 // A map {dim, tokens, heads, batch} of K or V, boxes of 64 x box_rows.  Heads or
 // batches that share one copy (stride 0) become one.
@@ -877,26 +920,26 @@ int kv_map(CUtensorMap *map, const struct htpg_attention_params *p, const void *
   *batch_step = p->batch > 1 && stride[0] != 0;
   const uint64_t dims[4] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(p->kv_len),
                             static_cast<uint64_t>(*head_step ? p->kv_heads : 1), static_cast<uint64_t>(*batch_step ? p->batch : 1)};
-  const uint64_t strides[3] = {step_of(p->kv_len > 1, stride[1], p->head_dim), step_of(*head_step, stride[2], p->head_dim),
-                               step_of(*batch_step, stride[0], p->head_dim)};
+  const uint64_t strides[3] = {step_of(p->kv_len > 1, stride[1], p->head_dim, 2), step_of(*head_step, stride[2], p->head_dim, 2),
+                               step_of(*batch_step, stride[0], p->head_dim, 2)};
   const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
   return op_tensor_map(map, p->type, base, 4, dims, strides, box);
 }
 
-// A map {dim, packed heads, tokens, heads or groups, batch} of Q, boxes of 128
-// rows: 128 / pack tokens, each with `pack` heads.
-int q_map(CUtensorMap *map, const struct htpg_attention_params *p, const void *base, int pack, int *head_step,
-          int *batch_step) {
-  const int64_t *stride = p->q_stride;
+// A map {dim, packed heads, tokens, heads or groups, batch} of Q or the output,
+// boxes of 128 bytes x `rows` rows: rows / pack tokens, each with `pack` heads.
+int rows_map(CUtensorMap *map, const struct htpg_attention_params *p, const void *base, int type, const int64_t *stride,
+             int pack, int rows, int *head_step, int *batch_step) {
   *head_step = p->q_heads > pack && stride[2] != 0;
-  const int others = *head_step ? p->q_heads / pack : 1;
   *batch_step = p->batch > 1 && stride[0] != 0;
+  const int others = *head_step ? p->q_heads / pack : 1, bytes = type_bytes(type);
   const uint64_t dims[5] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(pack), static_cast<uint64_t>(p->q_len),
                             static_cast<uint64_t>(others), static_cast<uint64_t>(*batch_step ? p->batch : 1)};
-  const uint64_t strides[4] = {step_of(pack > 1, stride[2], p->head_dim), step_of(p->q_len > 1, stride[1], p->head_dim),
-                               step_of(others > 1, stride[2] * pack, p->head_dim), step_of(*batch_step, stride[0], p->head_dim)};
-  const uint32_t box[5] = {64, static_cast<uint32_t>(pack), static_cast<uint32_t>(128 / pack), 1, 1};
-  return op_tensor_map(map, p->type, base, 5, dims, strides, box);
+  const uint64_t strides[4] = {step_of(pack > 1, stride[2], p->head_dim, bytes), step_of(p->q_len > 1, stride[1], p->head_dim, bytes),
+                               step_of(others > 1, stride[2] * pack, p->head_dim, bytes),
+                               step_of(*batch_step, stride[0], p->head_dim, bytes)};
+  const uint32_t box[5] = {static_cast<uint32_t>(128 / bytes), static_cast<uint32_t>(pack), static_cast<uint32_t>(rows / pack), 1, 1};
+  return op_tensor_map(map, type, base, 5, dims, strides, box);
 }
 
 template <typename T, typename TO, int DP, int KT>
@@ -934,9 +977,16 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
     if (qe[i] > 1 && a.os[i] * sizeof(TO) % 32) t.wide = 0;
   CUtensorMap mq, mk, mv;
   int rc;
-  if ((rc = q_map(&mq, p, a.q, t.pack, &t.q_head, &t.q_batch)) || (rc = kv_map(&mk, p, a.k, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
+  if ((rc = rows_map(&mq, p, a.q, p->type, p->q_stride, t.pack, 128, &t.q_head, &t.q_batch)) || (rc = kv_map(&mk, p, a.k, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
       (rc = kv_map(&mv, p, a.v, p->v_stride, KT, &t.v_head, &t.v_batch)))
     return rc;
+  // the output's, where a warp's 32 rows are whole tokens and no two rows are one
+  CUtensorMap mo = mq;
+  int own_head = 0, own_batch = 0;
+  if (tile_staged<TO>(DP) && t.pack <= 32) {
+    if ((rc = rows_map(&mo, p, a.out, p->out_type, p->out_stride, t.pack, 32, &own_head, &own_batch))) return rc;
+    t.staged = (own_head || p->q_heads == t.pack) && (own_batch || p->batch == 1);
+  }
   std::unique_lock<std::mutex> lock;
   if (t.splits > 1) {
     lock = op_lock();
@@ -949,11 +999,11 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
     t.part_o = reinterpret_cast<float *>(scratch + ml);
   }
   auto *fn = attn_tile_kernel<T, TO, DP, KT>;
-  using L = TileSmem<DP, KT>;
+  using L = TileSmem<DP, KT, tile_staged<TO>(DP)>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return op_result(e);
   e = op_launch(fn, dim3(static_cast<unsigned>(std::min(t.items, d.sms))), kTileThreads, L::kBytes, st, mq, mk,
-                mv, t);
+                mv, mo, t);
   if (e == cudaSuccess && t.splits > 1)
     e = op_launch(attn_join_kernel<TO>, dim3((t.units - t.whole) * 32), 256, 0, st, t);
   return op_result(e);

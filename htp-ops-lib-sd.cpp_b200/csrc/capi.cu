@@ -1178,7 +1178,9 @@ int op_tensor_map(CUtensorMap *map, int type, const void *base, int rank, const 
   for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
   const CUresult r = g_encode(map,
-                              type == HTPG_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                              type == HTPG_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                              : type == HTPG_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                               rank, const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

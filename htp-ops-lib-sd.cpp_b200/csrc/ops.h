@@ -36,7 +36,7 @@ std::unique_lock<std::mutex> op_lock();
 // captured graph may refer to is never freed.
 constexpr int kOpCounters = 16384;
 int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch);
-// Tensor map of a 16-bit array of `rank` <= 5 dimensions (innermost first;
+// Tensor map of an array (any HTPG_TYPE_*) of `rank` <= 5 dimensions (innermost first;
 // strides in bytes of dimensions 1 .. rank - 1), zero fill, 128-byte swizzle.
 int op_tensor_map(CUtensorMap *map, int type, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
                   const uint32_t *box);
