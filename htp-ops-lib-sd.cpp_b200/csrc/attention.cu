@@ -428,11 +428,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         bool dead = r < KT && r >= keys;
         if (bias) {
           // one key per thread: in units of log2, the lowest finite bias kept
-          // finite; two buffers, so that one barrier a tile is enough
+          // finite; two buffers, taken in turn over all steps (a thread may be
+          // one barrier ahead of the slowest reader), so one barrier a step is enough
           float add = r < keys ? ld_dep(bias + k0 + r) : -INFINITY;
           dead = r < KT && add == -INFINITY;
           if (!dead) add = fmaxf(add * kLog2e, -3.402823466e38f);
-          if (r < KT) bias_s[(j & 1) * KT + r] = add;
+          if (r < KT) bias_s[(seen & 1) * KT + r] = add;
           named_bar_sync(1 + w, 128);
         }
         const uint32_t buf = seen % NB, s_at = s_at0 + buf * KT;
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_ld_wait();
           // What takes no part becomes -inf; with a bias the scores come in units of log2.
           if (bias) {
-            const float4 *add = reinterpret_cast<const float4 *>(bias_s + (j & 1) * KT);
+            const float4 *add = reinterpret_cast<const float4 *>(bias_s + (~seen & 1) * KT);  // seen: counted on
 #pragma unroll
             for (int x = 0; x < KT / 2; x += 2) {
               const float4 y = add[x / 2];
@@ -506,8 +507,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               sum4[x % 4] = add2(sum4[x % 4], p);
               w32[x] = pack2<T>(p.x, p.y);
               if (kParts) {
-                const float2 back = unpack2<T>(w32[x]);
-                w32[16 + x] = pack2<T>(p.x - back.x, p.y - back.y);
+                const float2 rest = fma2(unpack2<T>(w32[x]), make_float2(-1.0f, -1.0f), p);
+                w32[16 + x] = pack2<T>(rest.x, rest.y);
               }
             }
             if (kParts)
