@@ -688,7 +688,8 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t at) {
                : "memory");
 }
 
-template <typename T, typename TO, int DB>
+// FULL: heads of exactly DB elements (a lane then always copies the same pieces).
+template <typename T, typename TO, int DB, bool FULL>
 __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __grid_constant__ FewArgs f) {
   using S = FewSmem<DB>;
   constexpr int KS = DB / 16, NS = S::kStages;
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % f.splits, unit = blockIdx.x / f.splits;
   const int kvh = unit % f.kv_heads, b = unit / f.kv_heads;
-  const int rows = a.q_len * a.group, n = clamped_len(a, b), dim = a.dim;
+  const int rows = a.q_len * a.group, n = clamped_len(a, b), dim = FULL ? DB : a.dim;
   const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const float *bias = a.bias ? a.bias + b * a.bias_stride : nullptr;
@@ -716,13 +717,27 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
       if (bias && in) in = ld_dep(bias + key0 + lane) != -INFINITY;
       const uint32_t live = __ballot_sync(0xffffffffu, in);
       uint8_t *ks = ring + slot * S::kStage, *vs = ks + kFewKeys * S::kPitch;
-      for (int i = lane; i < kFewKeys * f.unit16; i += 32) {
-        const int row = i * f.magic >> 16, piece = i - row * f.unit16;
-        const bool take = (live >> row & 1u) && piece * 8 < dim;
-        const long long key = take ? key0 + row : 0;
-        const int d = take ? piece * 8 : 0;
-        copy16(ks + row * S::kPitch + piece * 16, k + key * a.ks[1] + d, take);
-        copy16(vs + row * S::kPitch + piece * 16, v + key * a.vs[1] + d, take);
+      if constexpr (FULL) {
+        constexpr int kUnit = DB / 8, kRows = 32 / kUnit;  // pieces of a row, rows of one pass
+        const int row0 = lane / kUnit, d = lane % kUnit * 8;
+        const T *kp = k + static_cast<long long>(key0 + row0) * a.ks[1] + d, *vp = v + static_cast<long long>(key0 + row0) * a.vs[1] + d;
+        const uint32_t to = row0 * S::kPitch + d * 2;
+#pragma unroll
+        for (int i = 0; i < kFewKeys / kRows; ++i) {
+          const bool take = live >> (row0 + i * kRows) & 1u;
+          copy16(ks + to + i * kRows * S::kPitch, take ? kp : k, take);
+          copy16(vs + to + i * kRows * S::kPitch, take ? vp : v, take);
+          kp += kRows * a.ks[1], vp += kRows * a.vs[1];
+        }
+      } else {
+        for (int i = lane; i < kFewKeys * f.unit16; i += 32) {
+          const int row = i * f.magic >> 16, piece = i - row * f.unit16;
+          const bool take = (live >> row & 1u) && piece * 8 < dim;
+          const long long key = take ? key0 + row : 0;
+          const int d = take ? piece * 8 : 0;
+          copy16(ks + row * S::kPitch + piece * 16, k + key * a.ks[1] + d, take);
+          copy16(vs + row * S::kPitch + piece * 16, v + key * a.vs[1] + d, take);
+        }
       }
     }
     copy_commit();
@@ -771,19 +786,26 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
       mma_16<T>(s[1], q[x], m[1], m[3]);
     }
     const int key0 = chunk * kFewKeys;
+    if (bias || key0 + kFewKeys > n) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int key = key0 + 8 * h + 2 * t + e;
-        float add = key < n ? 0.0f : -INFINITY;
-        if (bias && key < n) {
-          add = ld_dep(bias + key);
-          if (add != -INFINITY) add = fmaxf(add * kLog2e, -3.402823466e38f);  // the lowest finite bias stays finite
+        for (int e = 0; e < 2; ++e) {
+          const int key = key0 + 8 * h + 2 * t + e;
+          float add = key < n ? 0.0f : -INFINITY;
+          if (bias && key < n) {
+            add = ld_dep(bias + key);
+            if (add != -INFINITY) add = fmaxf(add * kLog2e, -3.402823466e38f);  // the lowest finite bias stays finite
+          }
+          s[h][e] = add == -INFINITY ? -INFINITY : fmaf(s[h][e], c, add);
+          s[h][2 + e] = add == -INFINITY ? -INFINITY : fmaf(s[h][2 + e], c, add);
         }
-        s[h][e] = add == -INFINITY ? -INFINITY : fmaf(s[h][e], c, add);
-        s[h][2 + e] = add == -INFINITY ? -INFINITY : fmaf(s[h][2 + e], c, add);
-      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[h][e] *= c;
+    }
     float keep[2];
     bool moved = false;
 #pragma unroll
@@ -1024,7 +1046,7 @@ __global__ void __launch_bounds__(256) attn_zero_kernel(AttnArgs a, int out_byte
   }
 }
 
-template <typename T, typename TO, int DB>
+template <typename T, typename TO, int DB, bool FULL>
 int run_few(const struct htpg_attention_params *p, const AttnArgs &a, const OpDevice &d, cudaStream_t st) {
   using S = FewSmem<DB>;
   FewArgs f = {};
@@ -1056,7 +1078,7 @@ int run_few(const struct htpg_attention_params *p, const AttnArgs &a, const OpDe
     f.part_ml = reinterpret_cast<float2 *>(scratch);
     f.part_o = reinterpret_cast<float *>(scratch + ml);
   }
-  auto *fn = attn_few_kernel<T, TO, DB>;
+  auto *fn = attn_few_kernel<T, TO, DB, FULL>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
   if (e != cudaSuccess) return op_result(e);
   return op_result(op_launch(fn, dim3(static_cast<unsigned>(units * f.splits)), kFewWarps * 32, S::kBytes, st, f));
@@ -1070,9 +1092,11 @@ int run_attention(const struct htpg_attention_params *p, const AttnArgs &a, cons
                                0, st, a, static_cast<int>(sizeof(TO))));
   }
   if (static_cast<long long>(a.q_len) * a.group <= kFewRows) {
-    if (a.dim <= 64) return run_few<T, TO, 64>(p, a, d, st);
-    if (a.dim <= 128) return run_few<T, TO, 128>(p, a, d, st);
-    return run_few<T, TO, 192>(p, a, d, st);
+    if (a.dim == 64) return run_few<T, TO, 64, true>(p, a, d, st);
+    if (a.dim == 128) return run_few<T, TO, 128, true>(p, a, d, st);
+    if (a.dim <= 64) return run_few<T, TO, 64, false>(p, a, d, st);
+    if (a.dim <= 128) return run_few<T, TO, 128, false>(p, a, d, st);
+    return run_few<T, TO, 192, false>(p, a, d, st);
   }
   if (a.dim <= 64) return run_tiles<T, TO, 64, 64>(p, a, d, st);
   if (a.dim <= 128) return run_tiles<T, TO, 128, 64>(p, a, d, st);
