@@ -907,16 +907,31 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
   __threadfence();
   for (int r = warp; r < rows; r += kFewWarps) {
     const long long at = static_cast<long long>(unit) * f.splits * kFewRows + r;
-    float m = -INFINITY, l = 0.0f;
-    for (int x = 0; x < f.splits; ++x) m = fmaxf(m, __ldcg(&f.part_ml[at + x * kFewRows].x));
+    // the ranges' maxima and sums, two per lane, then their weighted rows
+    float2 ml[2];
+    float m = -INFINITY, l = 0.0f, weight[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int x = lane + 32 * i;
+      ml[i] = x < f.splits ? __ldcg(&f.part_ml[at + x * kFewRows]) : make_float2(-INFINITY, 0.0f);
+      m = fmaxf(m, ml[i].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      weight[i] = ex2_approx(ml[i].x - from);
+      l += weight[i] * ml[i].y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     float y[DB / 32];
 #pragma unroll
     for (int j = 0; j < DB / 32; ++j) y[j] = 0.0f;
+#pragma unroll 8
     for (int x = 0; x < f.splits; ++x) {
-      const float2 ml = __ldcg(&f.part_ml[at + x * kFewRows]);
-      const float w = ex2_approx(ml.x - from);
-      l += w * ml.y;
+      const float w = __shfl_sync(0xffffffffu, x < 32 ? weight[0] : weight[1], x & 31);
 #pragma unroll
       for (int j = 0; j < DB / 32; ++j) {
         const int d = lane + 32 * j;
