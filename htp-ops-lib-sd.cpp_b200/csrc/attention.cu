@@ -1072,14 +1072,17 @@ int run_few(const struct htpg_attention_params *p, const AttnArgs &a, const OpDe
   const long long units = static_cast<long long>(a.batch) * p->kv_heads;
   if (units > (1 << 30)) return HTPG_ECAPACITY;
   const int chunks = (a.kv_len + kFewKeys - 1) / kFewKeys;
-  // Key ranges: as many as make the rounds of CTAs (two per SM) shortest, a
-  // CTA's set-up and joining counted as two chunks per warp.
+  // Key ranges: as many as make the rounds of CTAs (two per SM) shortest, in
+  // chunks per warp; set-up counts as 2 chunks, with several ranges as 6 and half
+  // a chunk for each that is joined (one request, 32 heads over 8192 keys: 16
+  // ranges 12.8 us, 37 ranges, a CTA on every slot, 14.9; 16 requests over 1500:
+  // 1, 2, 3 ranges 23, 21, 25 us).
   const long long slots = 2LL * d.sms;
   f.splits = 1;
   long long least = -1;
   for (int s = 1; s <= 64 && (s == 1 || (units * s <= 4 * slots && s * kFewWarps <= chunks)); ++s) {
     const int per = (chunks + s - 1) / s;
-    const long long cost = (units * s + slots - 1) / slots * ((per + kFewWarps - 1) / kFewWarps + 2);
+    const long long cost = (units * s + slots - 1) / slots * ((per + kFewWarps - 1) / kFewWarps + (s > 1 ? 6 : 2)) * 4 + (s > 1 ? 2 * s : 0);
     if (least < 0 || cost < least) least = cost, f.splits = s;
   }
   f.per = (chunks + f.splits - 1) / f.splits;

@@ -117,14 +117,14 @@ struct DownSmem {
 };
 
 // Partial sums over K range blockIdx.y of t = x A^T for a tile's blocks
-// blockIdx.z, + gridDim.z, ...: part[range][row][max_rank].  A warp has 16 rows
-// and every fourth or eighth 32-element step of the range (four warps for each
-// half of a block with more than 16 rows); within a step lane t of a quad holds
-// elements 8t .. 8t + 7 of its rows of x and of A (any order of k will do, as
-// long as both sides have it).  x = hi + lo, hi with the 11 significant bits
-// that TF32 keeps, lo the rest, which TF32 cuts to 11 more; A is exact in TF32.
-// The tensor core's own sums round towards zero, so they are added up outside
-// of it every step.
+// blockIdx.z, + gridDim.z, ...: part[range][row][max_rank].  Up to eight blocks
+// at once: the warps are shared out evenly, and a block's warps (with more than
+// 16 rows: those of each half) take turns at the range's 32-element steps; within
+// a step lane t of a quad holds elements 8t .. 8t + 7 of its rows of x and of A
+// (any order of k will do, as long as both sides have it).  x = hi + lo, hi with
+// the 11 significant bits that TF32 keeps, lo the rest, which TF32 cuts to 11
+// more; A is exact in TF32.  The tensor core's own sums round towards zero, so
+// they are added up outside of it every step.
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, RK >= 64 ? 1 : 2)
     lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range) {
@@ -141,98 +141,118 @@ __global__ void __launch_bounds__(kLoraThreads, RK >= 64 ? 1 : 2)
   part += static_cast<long long>(blockIdx.y) * p.m * p.max_rank;
   uint4 *ring = smem + warp * (NS * S::kPieces * 32) + lane;
   float4 *red = reinterpret_cast<float4 *>(smem);
-  for (int block = blockIdx.z; block < rb.blocks; block += gridDim.z) {
-    const int start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
-    if (rank == 0) continue;
-    const bool halves = count > 16;
-    const int row_a = (halves ? (warp & 1) * 16 : 0) + g, row_b = row_a + 8;  // of the block
-    const T *a = static_cast<const T *>(p.a) + static_cast<long long>(rb.adapter[block]) * p.max_rank * p.k +
-                 static_cast<long long>(g) * p.k;
-    const float *xa = p.x + (row0 + rb.row[start + min(row_a, count - 1)]) * p.ldx;
-    const float *xb = p.x + (row0 + rb.row[start + min(row_b, count - 1)]) * p.ldx;
-    const int k_first = k0 + (halves ? warp >> 1 : warp) * 32 + 8 * t, k_step = halves ? 128 : 256;
-    const long long a_step = 8LL * p.k;
-    auto load = [&](int k, int slot) {
-      const bool in = k < k1;
-      uint4 *to = ring + slot * (S::kPieces * 32);
-      copy16(to, xa + (in ? k : 0), in);
-      copy16(to + 32, xa + (in ? k + 4 : 0), in);
-      copy16(to + 64, xb + (in ? k : 0), in);
-      copy16(to + 96, xb + (in ? k + 4 : 0), in);
-      const T *from = a + (in ? k : 0);
-#pragma unroll
-      for (int j = 0; j < NT; ++j, from += a_step) {
-        const bool rank_in = in && 8 * j + g < rank;
-        copy16(to + (4 + j) * 32, rank_in ? from : a, rank_in);
-      }
-      copy_commit();
-    };
+  const int z = blockIdx.z, zs = gridDim.z, mine = (rb.blocks - z + zs - 1) / zs;
+  auto store = [&](int start, int count, int place, int r, float x, float y) {
+    if (place < count && r < p.max_rank)
+      *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place]) * p.max_rank + r) = make_float2(x, y);
+  };
+  for (int done = 0; done < mine;) {
+    int group = kLoraWarps;  // warps per block
+    while (group > 1 && kLoraWarps / group < mine - done) group >>= 1;
+    const int at = done + warp / group, in_group = warp % group, block = z + at * zs;
+    const bool live = at < mine;
+    const int start = live ? rb.start[block] : 0, count = live ? rb.count[block] : 0, rank = live ? rb.rank[start] : 0;
+    const bool halves = count > 16, side = halves && group > 1;  // side: both halves of the rows at once
+    const T *a = static_cast<const T *>(p.a) + static_cast<long long>(g) * p.k;
+    if (rank) a += static_cast<long long>(rb.adapter[block]) * p.max_rank * p.k;
     float sum[NT][4];
+    for (int turn = 0; turn < (halves && !side ? 2 : 1); ++turn) {
+      const int half = side ? in_group & 1 : turn, place = half * 16 + g;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.0f;
+      for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.0f;
+      if (rank) {
+        const float *xa = p.x + (row0 + rb.row[start + min(place, count - 1)]) * p.ldx;
+        const float *xb = p.x + (row0 + rb.row[start + min(place + 8, count - 1)]) * p.ldx;
+        const int k_first = k0 + (side ? in_group >> 1 : in_group) * 32 + 8 * t, k_step = (side ? group / 2 : group) * 32;
+        const long long a_step = 8LL * p.k;
+        auto load = [&](int k, int slot) {
+          const bool in = k < k1;
+          uint4 *to = ring + slot * (S::kPieces * 32);
+          copy16(to, xa + (in ? k : 0), in);
+          copy16(to + 32, xa + (in ? k + 4 : 0), in);
+          copy16(to + 64, xb + (in ? k : 0), in);
+          copy16(to + 96, xb + (in ? k + 4 : 0), in);
+          const T *from = a + (in ? k : 0);
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) load(k_first + i * k_step, i);
-    int slot = 0;
-    for (int k = k_first; k - 8 * t < k1; k += k_step) {
-      load(k + (NS - 1) * k_step, slot == 0 ? NS - 1 : slot - 1);
-      copy_wait<NS - 1>();
-      const uint4 *from = ring + slot * (S::kPieces * 32);
-      slot = slot + 1 == NS ? 0 : slot + 1;
-      float c[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // elements 4h .. 4h + 3 of the lane's eight
-        const float4 va = *reinterpret_cast<const float4 *>(from + h * 32), vb = *reinterpret_cast<const float4 *>(from + (2 + h) * 32);
-        uint2 w[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = reinterpret_cast<const uint2 *>(from + (4 + j) * 32)[h];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // a0, a1: rows g, g + 8 of element 2e; a2, a3: of element 2e + 1
-          const float f[4] = {e ? va.z : va.x, e ? vb.z : vb.x, e ? va.w : va.y, e ? vb.w : vb.y};
-          uint32_t xh[4], xl[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            xh[y] = __float_as_uint(f[y]) & 0xffffe000u;
-            xl[y] = __float_as_uint(f[y] - __uint_as_float(xh[y]));
+          for (int j = 0; j < NT; ++j, from += a_step) {
+            const bool rank_in = in && 8 * j + g < rank;
+            copy16(to + (4 + j) * 32, rank_in ? from : static_cast<const T *>(p.a), rank_in);
           }
-          float2 b[NT];
+          copy_commit();
+        };
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            b[j] = unpack2<T>(e ? w[j].y : w[j].x);
-            mma_tf32(c[j], xl, __float_as_uint(b[j].x), __float_as_uint(b[j].y));
+        for (int i = 0; i < NS - 1; ++i) load(k_first + i * k_step, i);
+        int slot = 0;
+        for (int k = k_first; k - 8 * t < k1; k += k_step) {
+          load(k + (NS - 1) * k_step, slot == 0 ? NS - 1 : slot - 1);
+          copy_wait<NS - 1>();
+          const uint4 *from = ring + slot * (S::kPieces * 32);
+          slot = slot + 1 == NS ? 0 : slot + 1;
+          float c[NT][4];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // elements 4h .. 4h + 3 of the lane's eight
+            const float4 va = *reinterpret_cast<const float4 *>(from + h * 32);
+            const float4 vb = *reinterpret_cast<const float4 *>(from + (2 + h) * 32);
+            uint2 w[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) w[j] = reinterpret_cast<const uint2 *>(from + (4 + j) * 32)[h];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // a0, a1: rows g, g + 8 of element 2e; a2, a3: of element 2e + 1
+              const float f[4] = {e ? va.z : va.x, e ? vb.z : vb.x, e ? va.w : va.y, e ? vb.w : vb.y};
+              uint32_t xh[4], xl[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                xh[y] = __float_as_uint(f[y]) & 0xffffe000u;
+                xl[y] = __float_as_uint(f[y] - __uint_as_float(xh[y]));
+              }
+              float2 b[NT];
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                b[j] = unpack2<T>(e ? w[j].y : w[j].x);
+                mma_tf32(c[j], xl, __float_as_uint(b[j].x), __float_as_uint(b[j].y));
+              }
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma_tf32(c[j], xh, __float_as_uint(b[j].x), __float_as_uint(b[j].y));
+            }
           }
 #pragma unroll
-          for (int j = 0; j < NT; ++j) mma_tf32(c[j], xh, __float_as_uint(b[j].x), __float_as_uint(b[j].y));
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) sum[j][y] += c[j][y];
+        }
+        copy_wait<0>();
+      }
+      if (group == 1 && rank) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          store(start, count, place, 8 * j + 2 * t, sum[j][0], sum[j][1]);
+          store(start, count, place + 8, 8 * j + 2 * t, sum[j][2], sum[j][3]);
         }
       }
+    }
+    if (group > 1) {
+      __syncthreads();  // the rings become the warps' sums, added in order
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) sum[j][y] += c[j][y];
-    }
-    copy_wait<0>();
-    __syncthreads();  // the rings become the warps' sums, added in order
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-      red[(warp * NT + j) * 32 + lane] = make_float4(sum[j][0], sum[j][1], sum[j][2], sum[j][3]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < (halves ? 2 : 1) * NT * 32; i += kLoraThreads) {
-      const int h = i / (NT * 32), j = i / 32 % NT, l = i % 32;
-      float4 o = make_float4(0, 0, 0, 0);
-      for (int w = h; w < kLoraWarps; w += halves ? 2 : 1) {
-        const float4 v = red[(w * NT + j) * 32 + l];
-        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        red[(warp * NT + j) * 32 + lane] = make_float4(sum[j][0], sum[j][1], sum[j][2], sum[j][3]);
+      __syncthreads();
+      // the block's own warps add: fragment i of half i / (32 NT)
+      for (int i = in_group * 32 + lane; rank && i < (side ? 2 : 1) * NT * 32; i += group * 32) {
+        const int h = i / (NT * 32), j = i / 32 % NT;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int w = h; w < group; w += side ? 2 : 1) {
+          const float4 v = red[((warp - in_group + w) * NT + j) * 32 + lane];
+          o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        }
+        store(start, count, h * 16 + g, 8 * j + 2 * t, o.x, o.y);
+        store(start, count, h * 16 + g + 8, 8 * j + 2 * t, o.z, o.w);
       }
-      const int r = 8 * j + 2 * (l & 3), place = h * 16 + (l >> 2);
-      if (r >= p.max_rank) continue;
-      if (place < count)
-        *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place]) * p.max_rank + r) = make_float2(o.x, o.y);
-      if (place + 8 < count)
-        *reinterpret_cast<float2 *>(part + static_cast<long long>(row0 + rb.row[start + place + 8]) * p.max_rank + r) = make_float2(o.z, o.w);
+      __syncthreads();
     }
-    __syncthreads();
+    done += kLoraWarps / group;
   }
 }
 
@@ -271,7 +291,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   using S = UpSmem<T, RK>;
   constexpr int TM = S::TM, PITCH = S::PITCH, PARTS = S::PARTS, D = S::kDepth;
   __shared__ RowBlocks<TM> rb;
-  __shared__ float undo[TM];
+  __shared__ float undo[TM], shared_sums[kLoraWarps][(RK + 31) / 32 * 32];
   extern __shared__ __align__(16) uint4 smem[];
   __shared__ __align__(16) T ts[PARTS][TM][PITCH];
   // what the kernel before the down pass wrote is visible: that pass waited for
@@ -308,22 +328,67 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
 #pragma unroll
   for (int i = 0; i < D - 1; ++i) fetch(i);
   {
-    // one warp per place, every eighth, all of a warp's loads in flight together
+    // one warp per place, every eighth, a warp's loads of four ranges in flight together
     constexpr int PLACES = TM / kLoraWarps, NV = (RK + 31) / 32;
     const int rows = min(TM, p.m - row0);
+    const long long range_step = static_cast<long long>(p.m) * p.max_rank;
+    const float *src = part + static_cast<long long>(row0) * p.max_rank + lane;
     float v[PLACES][NV];
+#pragma unroll
+    for (int u = 0; u < PLACES; ++u)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) v[u][j] = 0.0f;
+    if (rows <= kLoraWarps / 2) {
+      // fewer places than warps: several warps share a place's ranges, and the
+      // place's own warp adds their sums in order
+      const int share = kLoraWarps / (rows <= 1 ? 1 : rows <= 2 ? 2 : 4), at = warp / share, rank = at < rows ? rb.rank[at] : 0;
+      float sum[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) sum[j] = 0.0f;
+#pragma unroll 4
+      for (int range = warp % share; range < ranges; range += share)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (lane + 32 * j < rank) sum[j] += src[range * range_step + rb.row[at] * p.max_rank + 32 * j];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) shared_sums[warp][lane + 32 * j] = sum[j];
+      __syncthreads();
+      if (warp < rows)
+        for (int w = warp * share; w < (warp + 1) * share; ++w)
+#pragma unroll
+          for (int j = 0; j < NV; ++j) v[0][j] += shared_sums[w][lane + 32 * j];
+    } else {
+      int offset[PLACES], rank[PLACES];
+#pragma unroll
+      for (int u = 0; u < PLACES; ++u) {
+        const int at = warp + kLoraWarps * u;
+        rank[u] = at < rows ? rb.rank[at] : 0;
+        offset[u] = rank[u] ? rb.row[at] * p.max_rank : 0;
+      }
+      const int used = (rows + kLoraWarps - 1) / kLoraWarps;  // places of a warp
+      if (used <= 2) {
+#pragma unroll 8
+        for (int range = 0; range < ranges; ++range, src += range_step)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+              if (lane + 32 * j < rank[u]) v[u][j] += src[offset[u] + 32 * j];
+      } else {
+#pragma unroll 2
+        for (int range = 0; range < ranges; ++range, src += range_step)
+#pragma unroll
+          for (int u = 0; u < PLACES; ++u)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+              if (lane + 32 * j < rank[u]) v[u][j] += src[offset[u] + 32 * j];
+      }
+    }
 #pragma unroll
     for (int u = 0; u < PLACES; ++u) {
       const int at = warp + kLoraWarps * u;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int r = lane + 32 * j;
-        v[u][j] = 0.0f;
-        if (at >= rows || r >= rb.rank[at]) continue;
-        const float *src = part + static_cast<long long>(row0 + rb.row[at]) * p.max_rank + r;
-        for (int range = 0; range < ranges; ++range) v[u][j] += src[static_cast<long long>(range) * p.m * p.max_rank];
-        v[u][j] *= rb.scale[at];
-      }
+      for (int j = 0; j < NV; ++j) v[u][j] = at < rows && lane + 32 * j < rb.rank[at] ? v[u][j] * rb.scale[at] : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < PLACES; ++u) {
@@ -448,8 +513,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
 
 template <typename T, int RK>
 int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
-  // Down: ranges of K until every SM has a block (none shorter than a step per
-  // warp), then blocks of one tile side by side.
+  // Down: ranges of K until every SM has a tile (none shorter than a step per
+  // warp), then a tile's blocks side by side.
   using U = UpSmem<T, RK>;
   using D = DownSmem<RK>;
   const int tiles = (p.m + 31) / 32, steps = (p.k + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
