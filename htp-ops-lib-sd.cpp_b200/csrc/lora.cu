@@ -21,6 +21,7 @@ struct LoraArgs {
   const void *a, *b;
   long long ldx, ldb, ldo;
   int m, k, n, adapters, max_rank;
+  int wide;  // rows of out are 32-byte aligned
 };
 
 constexpr int kLoraThreads = 256, kLoraWarps = 8;
@@ -282,8 +283,8 @@ struct UpSmem {
 // largest element in [2^10, 2^11) (undone at the end), so that what the parts
 // leave out is below 2^-22 of an element or 2^-35 of the row's largest; three for BF16.
 // Lane t of a quad holds ranks 8t .. 8t + 7 of each 32 (4t .. 4t + 3 of 16), and
-// columns 4t .. 4t + 3 of each 16 in two MMA tiles, so that B, base and out move
-// in 16-byte pieces.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
+// columns 8t .. 8t + 7 of 32 in four MMA tiles, so that B and base move in 16-byte
+// pieces and a row's 32 outputs are one 128-byte line of one store.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
 // flight in a ring of its own, read back by the lanes that copied them.
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, 2)
@@ -311,14 +312,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   auto fetch = [&](int item) {
     if (item < items && p.base) {
       const int block = z + f_block * zs, start = rb.start[block], count = rb.count[block];
-      const int c = c_first + f_group * (kLoraWarps * 32) + 4 * t;
+      const int c = c_first + f_group * (kLoraWarps * 32) + 8 * t;
       uint4 *to = ring + item % D * (4 * 32);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float *src = p.base + (row0 + rb.row[start + min(g + 8 * i, count - 1)]) * p.ldb;
         const bool ok = g + 8 * i < count;
         copy16(to + 2 * i * 32, src + (c < p.n ? c : 0), ok && c < p.n);
-        copy16(to + (2 * i + 1) * 32, src + (c + 16 < p.n ? c + 16 : 0), ok && c + 16 < p.n);
+        copy16(to + (2 * i + 1) * 32, src + (c < p.n ? c + 4 : 0), ok && c < p.n);
       }
       if (++f_block == mine) f_block = 0, ++f_group;
     }
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       const T *b = static_cast<const T *>(p.b) + static_cast<long long>(s) * p.n * p.max_rank;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int c = c0 + 16 * (j >> 1) + 4 * (g >> 1) + 2 * (j & 1) + (g & 1);
+        const int c = c0 + 8 * (g >> 1) + 2 * j + (g & 1);
         const T *row = b + static_cast<long long>(c) * p.max_rank + V * t;
 #pragma unroll
         for (int k = 0; k < NVEC; ++k) {
@@ -497,14 +498,18 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
           o[i][h].w = fmaf(acc[2 * h + 1][2 * i + 1], down[i], o[i][h].w);
         }
     }
+    const int c = c0 + 8 * t;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (g + 8 * i >= count) continue;
-      float *out = p.out + (row0 + rb.row[start + g + 8 * i]) * p.ldo;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = c0 + 16 * h + 4 * t;
-        if (c < p.n) __stcs(reinterpret_cast<float4 *>(out + c), o[i][h]);
+      if (g + 8 * i >= count || c >= p.n) continue;
+      float *out = p.out + (row0 + rb.row[start + g + 8 * i]) * p.ldo + c;
+      if (p.wide) {
+        asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "f"(o[i][0].x), "f"(o[i][0].y),
+                     "f"(o[i][0].z), "f"(o[i][0].w), "f"(o[i][1].x), "f"(o[i][1].y), "f"(o[i][1].z), "f"(o[i][1].w)
+                     : "memory");
+      } else {
+        __stcs(reinterpret_cast<float4 *>(out), o[i][0]);
+        __stcs(reinterpret_cast<float4 *>(out + 4), o[i][1]);
       }
     }
   }
@@ -599,6 +604,7 @@ extern "C" int htpg_lora_run(const struct htpg_lora_params *p, float *out, const
   r.n = p->n;
   r.adapters = p->adapters;
   r.max_rank = p->max_rank;
+  r.wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (p->m == 1 || r.ldo % 8 == 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   try {
     return p->type == HTPG_TYPE_F16 ? run_lora<__half>(r, d, st) : run_lora<__nv_bfloat16>(r, d, st);
