@@ -65,6 +65,7 @@ struct TileArgs {
   int wide;            // output rows are 32-byte aligned
   float *part_o;       // of split items: [item - whole][tile][128 rows][dim] sums
   float2 *part_ml;     // [item - whole][tile][128 rows] maximum (log2) and sum
+  float4 *sums;        // FP32 outputs over more than kFlush tiles: [CTA][tile][dim / 4][128 rows]
   uint32_t *watchdog;
 };
 
@@ -89,6 +90,16 @@ template <typename TO>
 constexpr bool tile_staged(int dp) {
   return sizeof(TO) == 4 && dp <= 128;
 }
+
+// FP32 outputs: the tensor core's sums round towards zero, which takes 2^-24 or
+// so of O away with every product and would show over thousands of keys. Every
+// kFlush key tiles O is added (to nearest) to sums in global memory, [dim / 4][row]
+// per CTA and tile, and begins anew. Four tiles keep the loss below what FP32
+// sums over thousands of keys lose anyway: 4096 queries over 4096 keys of 128,
+// error 5.2e-6 without, 1.7e-6 with eight, 1.1e-6 with four (FP32 products summed
+// in order: 1.4e-6). The sums stay in L2; four floats per atomic, 530 us
+// (one per atomic 677).
+constexpr int kFlush = 4;
 
 struct TileItem {
   int b, kvh, n, j0, j1, split;  // n keys take part, tiles [j0, j1) of them are this item's
@@ -300,7 +311,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // release them, this one at once where the item has no second tile.
       struct Step {
         int keys = 0;  // 0: none
-        bool mine = false, first = false, last = false;
+        bool mine = false, opens = false, first = false, last = false;
       } past[NB];
       uint32_t queries = 0, made = 0, taken = 0, n = 0;  // made, taken: steps of this tile
       TileItem it;
@@ -320,7 +331,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (open) {
           now.keys = min(KT, it.n - j * KT);
           now.mine = w == 0 || it.two;
-          now.first = j == it.j0;
+          now.first = kParts ? (j - it.j0) % kFlush == 0 : j == it.j0;  // O is overwritten
+          now.opens = j == it.j0;
           now.last = ++j == it.j1;
           open = !now.last;
         }
@@ -359,7 +371,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (now.keys) {
           const uint32_t k_slot = 2 * n % NS;
-          if (now.mine && now.first) ok = wait(q_full + 8 * w, queries++ & 1u);
+          if (now.mine && now.opens) ok = wait(q_full + 8 * w, queries++ & 1u);
           ok = ok && wait(kv_full + 8 * k_slot, 2 * n / NS & 1u);
           if (!ok) break;
           if (!now.mine) {
@@ -402,6 +414,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const bool wide = t.wide != 0;
     float *bias_s = reinterpret_cast<float *>(base + L::kBias) + w * 2 * KT;
     uint32_t seen = 0, used = 0;  // steps of this tile; slots passed
+    float4 *sums = kParts && t.sums ? t.sums + (static_cast<long long>(blockIdx.x) * 2 + w) * (dim / 4) * 128 + r : nullptr;
     bool ok = true;
     auto wait = [&](bool go, uint32_t bar, uint32_t parity) {
       const bool got = go && mbar_wait(bar, parity, t.watchdog, kWatchEpilogue, abort);
@@ -486,6 +499,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
                 tmem_st32(o_at + i, o);
               }
+              if (kParts && j > kFlush && keep != 1.0f) {
+#pragma unroll 4
+                for (int i = 0; i < dim / 4; ++i) {
+                  const float4 y = __ldcg(sums + i * 128);
+                  __stcg(sums + i * 128, make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep));
+                }
+              }
             }
           }
         }
@@ -520,6 +540,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           sum = sum4[0].x + sum4[0].y;
         }
         if (it.two && (w == 0 || j + 1 < nt)) named_bar_arrive(3 + 4 * (1 - w) + quad, 64);
+        if (kParts && j > 0 && j % kFlush == 0) {
+          // by now the product of the step before is done, and this step's waits for its weights
+          ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 2) % NB), (seen - 2) / NB & 1u);
+          tmem_st_wait();  // O as raised above
+#pragma unroll 1
+          for (int i = 0; ok && i < dim; i += 32) {
+            float o[32];
+            tmem_ld32(o_at + i, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+              if (i + x >= dim) break;
+              const float4 y = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+              float4 *at = sums + (i + x) / 4 * 128;
+              if (j == kFlush)
+                __stcg(at, y);
+              else
+                atomicAdd(at, y);  // this thread's alone, in order; nothing waits for its result
+            }
+          }
+        }
         if (!ok) continue;
         tmem_st_wait();
         tc_fence_before();
@@ -546,6 +587,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (nt) ok = wait(ok, pv_done + 16 * w + 8 * ((seen - 1) % NB), (seen - 1) / NB & 1u);
       if (!ok) continue;
+      auto load_o = [&](int i, float (&o)[32]) {  // 32 columns
+        tmem_ld32(o_at + i, o);
+        tmem_ld_wait();
+        if (kParts && nt > kFlush) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            if (i + x >= dim) break;
+            const float4 y = __ldcg(sums + (i + x) / 4 * 128);
+            o[x] += y.x, o[x + 1] += y.y, o[x + 2] += y.z, o[x + 3] += y.w;
+          }
+        }
+      };
       const bool none = sum == 0.0f;  // then O is zero, or there was no tile
       const bool split = item >= t.whole;
       const float inv = split || none ? 1.0f : 1.0f / sum;
@@ -561,10 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < dim; i += 32) {
           float o[32];
-          if (nt) {
-            tmem_ld32(o_at + i, o);
-            tmem_ld_wait();
-          }
+          if (nt) load_o(i, o);
           uint32_t words[32];
 #pragma unroll
           for (int x = 0; x < 32; ++x) words[x] = nt ? __float_as_uint(o[x] * inv) : 0u;
@@ -584,10 +634,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < dim; i += 32) {
           float o[32];
-          if (nt) {
-            tmem_ld32(o_at + i, o);
-            tmem_ld_wait();
-          }
+          if (nt) load_o(i, o);
 #pragma unroll
           for (int x = 0; x < 32; ++x) o[x] = nt ? o[x] * inv : 0.0f;
           if (mine) {
@@ -844,10 +891,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
       // transposed matrices: keys 0-7 and 8-15 of elements 0-7, then of 8-15
       uint32_t m[4];
       ldmatrix4t(m, vs + (lane & 15) * S::kPitch + x * 32 + (lane >> 4) * 16);
-      if (kParts) mma_16<T>(o[2 * x], lo, m[0], m[1]);
-      mma_16<T>(o[2 * x], hi, m[0], m[1]);
-      if (kParts) mma_16<T>(o[2 * x + 1], lo, m[2], m[3]);
-      mma_16<T>(o[2 * x + 1], hi, m[2], m[3]);
+      if (kParts) {
+        // the tensor core's sums round towards zero: added up outside of it
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_16<T>(y, lo, m[2 * h], m[2 * h + 1]);
+          mma_16<T>(y, hi, m[2 * h], m[2 * h + 1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[2 * x + h][e] += y[e];
+        }
+      } else {
+        mma_16<T>(o[2 * x], hi, m[0], m[1]);
+        mma_16<T>(o[2 * x + 1], hi, m[2], m[3]);
+      }
     }
     __syncwarp();  // every lane is done with the chunk before its slot is filled again
   }
@@ -1026,21 +1083,24 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
     t.staged = (own_head || p->q_heads == t.pack) && (own_batch || p->batch == 1);
   }
   std::unique_lock<std::mutex> lock;
-  if (t.splits > 1) {
+  const int grid = std::min(t.items, d.sms);
+  const bool flushes = sizeof(TO) == 4 && tiles > kFlush;
+  if (t.splits > 1 || flushes) {
     lock = op_lock();
     uint32_t *counters;
     uint8_t *scratch;
-    const size_t rows = static_cast<size_t>(t.items - t.whole) * 256, ml = rows * sizeof(float2);
-    rc = op_scratch(st, ml + rows * a.dim * 4, &counters, &scratch);
+    const size_t rows = static_cast<size_t>(t.items - t.whole) * 256, ml = rows * sizeof(float2), parts = rows * a.dim * 4;
+    rc = op_scratch(st, ml + parts + (flushes ? static_cast<size_t>(grid) * 256 * a.dim * 4 : 0), &counters, &scratch);
     if (rc) return rc;
     t.part_ml = reinterpret_cast<float2 *>(scratch);
     t.part_o = reinterpret_cast<float *>(scratch + ml);
+    if (flushes) t.sums = reinterpret_cast<float4 *>(scratch + ml + parts);
   }
   auto *fn = attn_tile_kernel<T, TO, DP, KT>;
   using L = TileSmem<DP, KT, tile_staged<TO>(DP)>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return op_result(e);
-  e = op_launch(fn, dim3(static_cast<unsigned>(std::min(t.items, d.sms))), kTileThreads, L::kBytes, st, mq, mk,
+  e = op_launch(fn, dim3(grid), kTileThreads, L::kBytes, st, mq, mk,
                 mv, mo, t);
   if (e == cudaSuccess && t.splits > 1)
     e = op_launch(attn_join_kernel<TO>, dim3((t.units - t.whole) * 32), 256, 0, st, t);
