@@ -1182,10 +1182,10 @@ int run_attention(const struct htpg_attention_params *p, const AttnArgs &a, cons
 }
 
 // 16-byte vectors along every dimension that is stepped along, forwards, and
-// within a tensor map's reach; tokens have rows of their own.
-bool strides_fit(const int64_t *s, const int (&extent)[3], int per16) {
+// within a tensor map's reach; tokens, and everything written, have rows of their own.
+bool strides_fit(const int64_t *s, const int (&extent)[3], int per16, bool written) {
   for (int i = 0; i < 3; ++i)
-    if (extent[i] > 1 && (s[i] % per16 || s[i] < (i == 1) || s[i] >= (int64_t{1} << 38))) return false;
+    if (extent[i] > 1 && (s[i] % per16 || s[i] < (i == 1 || written) || s[i] >= (int64_t{1} << 38))) return false;
   return true;
 }
 
@@ -1209,8 +1209,8 @@ extern "C" int htpg_cross_attention(const struct htpg_attention_params *p, void 
   if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
         reinterpret_cast<uintptr_t>(v)) & 15u) ||
       ((reinterpret_cast<uintptr_t>(kv_lens) | reinterpret_cast<uintptr_t>(key_bias)) & 3u) ||
-      !strides_fit(p->q_stride, qe, 8) || !strides_fit(p->k_stride, ke, 8) || !strides_fit(p->v_stride, ke, 8) ||
-      !strides_fit(p->out_stride, qe, 16 / type_bytes(p->out_type)))
+      !strides_fit(p->q_stride, qe, 8, false) || !strides_fit(p->k_stride, ke, 8, false) ||
+      !strides_fit(p->v_stride, ke, 8, false) || !strides_fit(p->out_stride, qe, 16 / type_bytes(p->out_type), true))
     return HTPG_ECONTROL;
   OpDevice d;
   const int rc = op_device(&d);

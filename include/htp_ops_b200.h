@@ -281,10 +281,12 @@ int htpg_qkv_rope(const struct htpg_rope_params *p, void *q_out, void *k_out, vo
  * stride 0 in k and v shares one encoder's states.  type: F16 or BF16 (q, k,
  * v); out_type: the same or F32.  The weights are rounded to `type` for the
  * product with V; with an F32 output they are carried in two parts (twice the
- * bits), so that the result is good to about 2^-21 (F16) or 2^-16 (BF16) of
- * the values.  head_dim: a multiple of 8 up to 192; q_heads a multiple of
- * kv_heads; scale > 0; pointers 16-byte aligned and q, k, v strides multiples
- * of 8 elements (out: 16 bytes) (HTPG_ECONTROL).  batch or q_len 0: nothing is
+ * bits) and summed in FP32, so that the result is good to a few 2^-20 (F16) or
+ * to about 2^-16 (BF16) of the largest value.  head_dim: a multiple of 8 up to
+ * 192; q_heads a multiple of kv_heads; scale > 0.  Pointers 16-byte aligned
+ * (kv_lens, key_bias: 4); along dimensions longer than one, strides are
+ * multiples of 8 elements (out: of 16 bytes), below 2^38, not negative, and not
+ * zero for tokens and in out (HTPG_ECONTROL).  batch or q_len 0: nothing is
  * done; kv_len 0: zeros. */
 struct htpg_attention_params {
   int32_t type, out_type; /* HTPG_TYPE_* */
@@ -308,7 +310,8 @@ int htpg_cross_attention(const struct htpg_attention_params *p, void *out, const
  * NULL (zeros).  All of row_adapter [m], ranks and scales [adapters] (int32,
  * int32, FP32) are device arrays.  x, base, out FP32 with row strides ldx, ldb,
  * ldo (0: dense); a, b of `type` (F16 or BF16).  FP32 accuracy: x and the
- * intermediate x A^T are split so that no bits that FP32 keeps are lost.
+ * intermediate x A^T are carried in parts of 22 bits or more together, and all
+ * sums are FP32.
  * k, n: multiples of 8; max_rank: a multiple of 8 up to 128; pointers 16-byte
  * aligned, ld* multiples of 4 (HTPG_ECONTROL).  m = 0: nothing is done. */
 struct htpg_lora_params {

@@ -87,6 +87,10 @@ def _attn(**change):
     ({}, dict(bias=A16 + 1), htpg.ECONTROL),
     (dict(q_stride=(768, 260, 64)), {}, htpg.ECONTROL), (dict(k_stride=(640, 128, 68)), {}, htpg.ECONTROL),
     (dict(v_stride=(644, 128, 64)), {}, htpg.ECONTROL), (dict(out_stride=(768, 258, 64)), {}, htpg.ECONTROL),
+    (dict(q_stride=(768, -256, 64)), {}, htpg.ECONTROL), (dict(k_stride=(-640, 128, 64)), {}, htpg.ECONTROL),
+    (dict(v_stride=(640, 128, -64)), {}, htpg.ECONTROL), (dict(k_stride=(640, 0, 64)), {}, htpg.ECONTROL),
+    (dict(q_stride=(1 << 38, 256, 64)), {}, htpg.ECONTROL), (dict(out_stride=(0, 256, 64)), {}, htpg.ECONTROL),
+    (dict(out_stride=(768, 256, 0)), {}, htpg.ECONTROL),
     (dict(batch=0), {}, htpg.OK), (dict(q_len=0), {}, htpg.OK),
 ])
 def test_cross_attention_refusals(lib, change, ptrs, code):
