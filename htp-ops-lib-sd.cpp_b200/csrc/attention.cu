@@ -52,6 +52,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct TileArgs {
   AttnArgs a;
   int pack;            // heads of a group that share a tile (rows token by token), a power of two, or 1
+  int log_pack;
   int row_tiles;       // tiles of one head, or of one group's heads together
   int tiles;           // tiles of one key/value head
   int pairs;           // tile pairs of one key/value head
@@ -137,7 +138,7 @@ __device__ __forceinline__ TileItem tile_item(const TileArgs &t, int item, const
   for (int w = 0; w < 2; ++w) {
     const uint32_t tile = 2 * pair + w, head = t.tiles == t.row_tiles ? 0 : tile / t.row_tiles;
     r.head[w] = r.kvh * t.a.group + head;
-    r.row0[w] = (tile - head * t.row_tiles) * (128 / t.pack);
+    r.row0[w] = (tile - head * t.row_tiles) * (128 >> t.log_pack);
   }
   return r;
 }
@@ -272,8 +273,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (elect_one()) {
             mbar_arrive_expect_tx(q_full + 8 * w, panels * 128 * 128);
             for (int p = 0; p < panels; ++p)
-              tma_load_5d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, 0, it.row0[w],
-                          (t.pack > 1 ? it.kvh : it.head[w]) * t.q_head, it.b * t.q_batch);
+              tma_load_5d(q_s + w * L::kQ + p * 128 * 128, &map_q, q_full + 8 * w, p * 64, 0, w ? it.row0[1] : it.row0[0],
+                          (t.pack > 1 ? it.kvh : w ? it.head[1] : it.head[0]) * t.q_head, it.b * t.q_batch);
           }
           ++tiles[w];
           // the first keys right after the first tile's queries
@@ -425,12 +426,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // iteration; after a wait that gave up they skip the work.
     for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
       const TileItem it = tile_item<KT>(t, item, lens);
+      const int row0 = w ? it.row0[1] : it.row0[0], head0 = w ? it.head[1] : it.head[0];
       const int nt = it.j1 - it.j0;
       if (w == 1 && !it.two) {
         used += 2 * nt;
         continue;
       }
-      const int token = it.row0[w] + r / t.pack, head = it.head[w] + r % t.pack;
+      const int token = row0 + (r >> t.log_pack), head = head0 + (r & (t.pack - 1));
       const bool mine = token < t.a.q_len;
       const float *bias = t.a.bias ? t.a.bias + it.b * t.a.bias_stride : nullptr;
       const float unit = bias ? 1.0f : c;  // of the scores in s[], in log2
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               for (int p = 0; p * 64 < dim; ++p)
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
-                  *reinterpret_cast<uint4 *>(base + 2 * L::kQ + v_slot * L::kStage + p * KT * 128 + r * 128 + x * 16) =
+                  *reinterpret_cast<uint4 *>(base + 2 * L::kQ + v_slot * L::kStage + p * KT * 128 + r * 128 + ((x ^ (r & 7)) << 4)) =
                       make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
           }
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // (which leaves out rows and columns past the ends): straight from the
         // threads, every store would touch 32 lines.
         const uint32_t stage = q_s + L::kOut + warp * 4096, at = stage + lane * 128;
-        const int first = it.row0[w] + quad * 32 / t.pack;
+        const int first = row0 + (quad * 32 >> t.log_pack);
 #pragma unroll 1
         for (int i = 0; i < dim; i += 32) {
           float o[32];
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (first < t.a.q_len && elect_one()) {
-            tma_store_5d(&map_out, stage, i, 0, first, t.pack > 1 ? it.kvh : it.head[w], it.b);
+            tma_store_5d(&map_out, stage, i, 0, first, t.pack > 1 ? it.kvh : head0, it.b);
             bulk_commit();
           }
         }
@@ -1044,6 +1046,7 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   // A group's heads share tiles where their number divides 128: few tokens then
   // fill a tile (16 tokens x 4 heads in one tile instead of four).
   t.pack = (a.group & (a.group - 1)) == 0 && a.group <= 128 && p->q_stride[2] != 0 ? a.group : 1;
+  while (1 << t.log_pack < t.pack) ++t.log_pack;
   t.kv_heads = p->kv_heads;
   const long long row_tiles = (static_cast<long long>(a.q_len) * t.pack + 127) / 128, tiles_kv = row_tiles * (a.group / t.pack);
   const long long pairs = (tiles_kv + 1) / 2;
