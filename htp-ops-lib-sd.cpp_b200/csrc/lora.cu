@@ -126,6 +126,10 @@ struct DownSmem {
 // the 11 significant bits that TF32 keeps, lo the rest, which TF32 cuts to 11
 // more; A is exact in TF32.  The tensor core's own sums round towards zero, so
 // they are added up outside of it every step.
+// Bound by instructions (16384 x 1536, rank 64: 65 us for 101 MB; the tensor pipe
+// 46 % busy, issue slots 38 %): x is split and A widened in registers.  Both halves
+// of 32 rows in one warp save A's second reading but leave 255 registers and less
+// in flight: 74 us.
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, RK >= 64 ? 1 : 2)
     lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range) {
@@ -273,6 +277,10 @@ struct UpSmem {
   static constexpr int kVec = RK >= 32 ? 8 : 4;  // ranks a lane holds together
   static constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
   static constexpr int kDepth = 4;  // blocks of base in flight per warp
+  // The next item's part of B is read ahead, the first before t (one row, 4096 x
+  // 14336: 8.6 -> 8.0 us; 16384 mixed rows of rank 16: 300 -> 283); above rank 32
+  // the registers do not reach.
+  static constexpr bool kAhead = RK <= 32;
   static constexpr int kBytes = kLoraWarps * kDepth * 4 * 32 * 16;
 };
 
@@ -284,8 +292,11 @@ struct UpSmem {
 // leave out is below 2^-22 of an element or 2^-35 of the row's largest; three for BF16.
 // Lane t of a quad holds ranks 8t .. 8t + 7 of each 32 (4t .. 4t + 3 of 16), and
 // columns 8t .. 8t + 7 of 32 in four MMA tiles, so that B and base move in 16-byte
-// pieces and a row's 32 outputs are one 128-byte line of one store.  Each warp keeps kDepth blocks (16 rows x 32 columns) of base in
-// flight in a ring of its own, read back by the lanes that copied them.
+// pieces and a row's 32 outputs are one 128-byte line of one store.  Each warp keeps
+// kDepth blocks (16 rows x 32 columns) of base in flight in a ring of its own, read
+// back by the lanes that copied them.
+// Bound by HBM through base and out: 16384 rows x 6144, rank 64: 165 us for 805 MB
+// (4.9 TB/s); few rows by the chain ids -> t -> out (one row, both passes: 8 us).
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, 2)
     lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range) {
@@ -325,6 +336,25 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
     }
     copy_commit();
   };
+  constexpr int V = S::kVec, NVEC = RK / (4 * V);  // vectors of V ranks per lane
+  using Vec = std::conditional_t<V == 8, uint4, uint2>;
+  // B's vectors for the 32 columns of one group, as they lie
+  auto take = [&](Vec (&w)[4][NVEC], int block, int group) {
+    const int rank = rb.rank[rb.start[block]];
+    const T *b = static_cast<const T *>(p.b) + static_cast<long long>(max(rb.adapter[block], 0)) * p.n * p.max_rank;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c_first + group * (kLoraWarps * 32) + 8 * (g >> 1) + 2 * j + (g & 1);
+      const T *row = b + static_cast<long long>(c) * p.max_rank + V * t;
+#pragma unroll
+      for (int k = 0; k < NVEC; ++k) {
+        w[j][k] = Vec{};
+        if (c < p.n && 4 * V * k + V * t < rank) w[j][k] = *reinterpret_cast<const Vec *>(row + 4 * V * k);
+      }
+    }
+  };
+  Vec w[4][NVEC], next[4][NVEC];
+  if (S::kAhead && items > 0) take(next, z, 0);
   grid_dependency_wait();
 #pragma unroll
   for (int i = 0; i < D - 1; ++i) fetch(i);
@@ -424,9 +454,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
     }
   }
   __syncthreads();
-  constexpr int V = S::kVec, NVEC = RK / (4 * V);  // vectors of V ranks per lane
-  using Vec = std::conditional_t<V == 8, uint4, uint2>;
-  Vec w[4][NVEC];
   int held = -1, held_group = -1, group = 0, at = 0;
   for (int item = 0; item < items; ++item) {
     fetch(item + D - 1);
@@ -434,16 +461,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
     const int s = rb.adapter[block], start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
     if (rank && (s != held || group != held_group)) {
       held = s, held_group = group;
-      const T *b = static_cast<const T *>(p.b) + static_cast<long long>(s) * p.n * p.max_rank;
+      if (S::kAhead) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = c0 + 8 * (g >> 1) + 2 * j + (g & 1);
-        const T *row = b + static_cast<long long>(c) * p.max_rank + V * t;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < NVEC; ++k) {
-          w[j][k] = Vec{};
-          if (c < p.n && 4 * V * k + V * t < rank) w[j][k] = *reinterpret_cast<const Vec *>(row + 4 * V * k);
-        }
+          for (int k = 0; k < NVEC; ++k) w[j][k] = next[j][k];
+      } else {
+        take(w, block, group);
       }
       if (rank % V) {  // what lies past the rank may be anything
 #pragma unroll
@@ -458,6 +482,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       }
     }
     if (++at == mine) at = 0, ++group;
+    if (S::kAhead && item + 1 < items && (rb.adapter[z + at * zs] != held || group != held_group)) take(next, z + at * zs, group);
     copy_wait<D - 1>();
     if (rank == 0 && in_place) continue;
     float4 o[2][2];
@@ -518,13 +543,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
 
 template <typename T, int RK>
 int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
-  // Down: ranges of K until every SM has a tile (none shorter than a step per
-  // warp), then a tile's blocks side by side.
+  // Down: ranges of K until every SM has a tile (multiples of 128, none shorter
+  // than a step per warp: 1000 mixed rows 21.5 us in all; multiples of 256 22.5;
+  // two CTAs per SM 23.9), then a tile's blocks side by side.
   using U = UpSmem<T, RK>;
   using D = DownSmem<RK>;
-  const int tiles = (p.m + 31) / 32, steps = (p.k + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
-  const int ranges = std::max(1, std::min(steps, d.sms / tiles));
-  const int k_range = (steps + ranges - 1) / ranges * kLoraWarps * 32;
+  const int tiles = (p.m + 31) / 32, parts = (p.k + 127) / 128;
+  const int ranges = std::max(1, std::min(parts / 2, d.sms / tiles));
+  const int k_range = (parts + ranges - 1) / ranges * 128;
   const int k_ranges = (p.k + k_range - 1) / k_range;
   const int z_down = std::max(1, std::min({8, p.adapters, p.m, d.sms / (tiles * k_ranges)}));
   // Up: the column ranges whose rounds of CTAs (two per SM) do least, a CTA's
