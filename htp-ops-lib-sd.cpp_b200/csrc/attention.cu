@@ -40,10 +40,20 @@ struct AttnArgs {
 // TMEM columns: per tile two buffers of S (64 each, P in place; one buffer for
 // heads above 128) and O (DP).  With two, the scores of the next two key tiles are
 // made while the softmax of one runs, so the chain scores -> softmax -> weights
-// never waits for the tensor core.  P is the A operand in TMEM; V, as loaded ([key][dim]), the
-// MN-major B operand.  The maximum is only raised (and O rescaled) once a score
-// passes it by 2^8: weights up to 2^8 (FP16: 2^15, see kShift) stay exact
-// enough and most tiles skip the rescale.
+// never waits for the tensor core.  P is the A operand in TMEM; V, as loaded
+// ([key][dim]), the MN-major B operand.
+// Rounding: scores and sums are FP32; the weights are rounded to the 16 bits of
+// the tensor core's A operand (with FP32 outputs the rest follows as a second
+// operand), the sum they are divided by is of the unrounded ones.  The maximum is
+// only raised (and O rescaled) once a score passes it by 2^kLazy, which changes
+// no weight's relative error and lets most tiles skip the rescale.
+// Bound by the issue of the softmax's instructions and the latency of one step's
+// chain, not by the tensor core: 4 x 4096 queries of 12 heads of 128 over 4096
+// keys, FP16: 407 us = 1010 TFLOP/s (0.61 of cuBLAS); 16384 over 512, BF16: 81 us.
+// 64 keys a tile: 128 with one buffer of S 611 us.  Turns at the exponentials 489
+// -> 455, one elected lane issuing 548 -> 489.  Few keys are bound by an item's
+// chain load -> scores -> weights -> output, about 3.5 us: 2 x 4096 queries of 24
+// heads of 64 over 77 keys 28.6 us.
 constexpr int kTileThreads = 384;
 constexpr int kLensHeld = 256;   // batches whose lengths are kept in shared memory
 constexpr float kLazy = 8.0f;    // log2 of how far a score may pass the held maximum
@@ -190,8 +200,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using L = TileSmem<DP, KT, kStaged>;
   // FP32 outputs: P in two 16-bit parts, high and low, each KT / 2 TMEM columns
   constexpr bool kParts = sizeof(TO) == 4;
-  // FP16 weights are 2^7 times larger, so that those below 2^-14 of the
-  // largest keep their bits; with kLazy they stay below 2^15
+  // FP16 weights are 2^7 times larger, so that those down to 2^-21 of the
+  // largest keep their 11 bits; with kLazy they stay at 2^15 or below
   constexpr float kShift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
   constexpr uint32_t kFormat = std::is_same<T, __half>::value ? 0u : 1u;
   constexpr uint32_t kIdesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | (8u << 24);  // F32 sums, M = 128
@@ -259,7 +269,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!wait(kv_empty + 8 * s, (loads / NS & 1u) ^ 1u)) return false;
         if (elect_one()) {
           mbar_arrive_expect_tx(bar, panels * KT * 128);
-          for (int p = 0; p < panels; ++p) tma_load_4d(kv_s + s * L::kStage + p * KT * 128, map, bar, p * 64, j * KT, h, b);
+          for (int p = 0; p < panels; ++p)
+            tma_load_4d(kv_s + s * L::kStage + p * KT * 128, map, bar, p * 64, j * KT, h, b);
         }
         ++loads;
         return true;
@@ -415,7 +426,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const bool wide = t.wide != 0;
     float *bias_s = reinterpret_cast<float *>(base + L::kBias) + w * 2 * KT;
     uint32_t seen = 0, used = 0;  // steps of this tile; slots passed
-    float4 *sums = kParts && t.sums ? t.sums + (static_cast<long long>(blockIdx.x) * 2 + w) * (dim / 4) * 128 + r : nullptr;
+    float4 *sums = nullptr;
+    if (kParts && t.sums) sums = t.sums + (static_cast<long long>(blockIdx.x) * 2 + w) * (dim / 4) * 128 + r;
     bool ok = true;
     auto wait = [&](bool go, uint32_t bar, uint32_t parity) {
       const bool got = go && mbar_wait(bar, parity, t.watchdog, kWatchEpilogue, abort);
@@ -466,7 +478,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int x = 0; x < KT / 2; x += 2) {
               const float4 y = add[x / 2];
               float2 &s0 = s[x / 16][x % 16], &s1 = s[x / 16][x % 16 + 1];
-              const float2 f0 = fma2(s0, make_float2(c, c), make_float2(y.x, y.y)), f1 = fma2(s1, make_float2(c, c), make_float2(y.z, y.w));
+              const float2 c2 = make_float2(c, c);
+              const float2 f0 = fma2(s0, c2, make_float2(y.x, y.y)), f1 = fma2(s1, c2, make_float2(y.z, y.w));
               s0 = make_float2(y.x == -INFINITY ? -INFINITY : f0.x, y.y == -INFINITY ? -INFINITY : f0.y);
               s1 = make_float2(y.z == -INFINITY ? -INFINITY : f1.x, y.w == -INFINITY ? -INFINITY : f1.y);
             }
@@ -481,7 +494,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           // Four running maxima and sums: one of each would be a chain of 64 dependent operations.
           float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int x = 0; x < KT / 2; ++x) most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[x / 16][x % 16].x, s[x / 16][x % 16].y));
+          for (int x = 0; x < KT / 2; ++x)
+            most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[x / 16][x % 16].x, s[x / 16][x % 16].y));
           const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3])) * unit;
           const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
           if (__any_sync(0xffffffffu, raise)) {
@@ -517,7 +531,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (it.two) named_bar_sync(3 + 4 * w + quad, 64);
         if (ok) {
           const float from = top == -INFINITY ? 0.0f : top - kShift;
-          float2 sum4[4] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          const float2 zero2 = make_float2(0.0f, 0.0f);
+          float2 sum4[4] = {make_float2(sum, 0.0f), zero2, zero2, zero2};
 #pragma unroll
           for (int h = 0; h < KT / 32; ++h) {
             if (32 * h >= keys) break;
@@ -575,12 +590,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const uint32_t v_slot = (used + 1) % NS;
             ok = wait(ok, kv_full + 8 * v_slot, (used + 1) / NS & 1u);
             if (!ok) continue;
-            if (dead)
+            if (dead) {
+              const uint32_t at = q_s + 2 * L::kQ + v_slot * L::kStage + r * 128;
               for (int p = 0; p * 64 < dim; ++p)
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                  *reinterpret_cast<uint4 *>(base + 2 * L::kQ + v_slot * L::kStage + p * KT * 128 + r * 128 + ((x ^ (r & 7)) << 4)) =
-                      make_uint4(0, 0, 0, 0);
+                for (int x = 0; x < 8; ++x)  // in an order that spreads neighbouring rows over the banks
+                  sts_u32x4(at + p * KT * 128 + ((x ^ (r & 7)) << 4), 0, 0, 0, 0);
+            }
             fence_proxy_async_smem();
           }
         }
@@ -701,7 +717,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 // are m16n8k16 products on rows of the ring (ldmatrix, transposed for V), with
 // a running maximum and sum per warp, joined at the end through shared
 // memory, and over the key ranges of a unit by its last CTA, in order.  Keys
-// that take no part are never copied: their rows are zeros.
+// that take no part are never copied: their rows are zeros.  Weights are rounded
+// as in the tiles above (two parts for FP32 outputs).
+// 16 requests, 32 heads in 8 groups of 128, over 1500 keys and fewer: 22 us for
+// 74 MB (3.4 TB/s; the wave's tail and the chain copy -> scores -> weights of each
+// warp's chunks, 25 % issue); one request over 8192 keys: 13 us for 34 MB.
 constexpr int kFewWarps = 4, kFewRows = 16, kFewKeys = 16;
 
 struct FewArgs {
@@ -769,7 +789,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
       if constexpr (FULL) {
         constexpr int kUnit = DB / 8, kRows = 32 / kUnit;  // pieces of a row, rows of one pass
         const int row0 = lane / kUnit, d = lane % kUnit * 8;
-        const T *kp = k + static_cast<long long>(key0 + row0) * a.ks[1] + d, *vp = v + static_cast<long long>(key0 + row0) * a.vs[1] + d;
+        const T *kp = k + static_cast<long long>(key0 + row0) * a.ks[1] + d;
+        const T *vp = v + static_cast<long long>(key0 + row0) * a.vs[1] + d;
         const uint32_t to = row0 * S::kPitch + d * 2;
 #pragma unroll
         for (int i = 0; i < kFewKeys / kRows; ++i) {
@@ -1007,7 +1028,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
 }
 
 // Stride (bytes) of an extent: its own where it is stepped along, any valid one otherwise.
-uint64_t step_of(bool stepped, int64_t stride, int dim, int bytes) { return static_cast<uint64_t>(stepped ? stride : dim) * bytes; }
+uint64_t step_of(bool stepped, int64_t stride, int dim, int bytes) {
+  return static_cast<uint64_t>(stepped ? stride : dim) * bytes;
+}
 
 // A map {dim, tokens, heads, batch} of K or V, boxes of 64 x box_rows.  Heads or
 // batches that share one copy (stride 0) become one.
@@ -1015,9 +1038,10 @@ int kv_map(CUtensorMap *map, const struct htpg_attention_params *p, const void *
            int *head_step, int *batch_step) {
   *head_step = p->kv_heads > 1 && stride[2] != 0;
   *batch_step = p->batch > 1 && stride[0] != 0;
-  const uint64_t dims[4] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(p->kv_len),
-                            static_cast<uint64_t>(*head_step ? p->kv_heads : 1), static_cast<uint64_t>(*batch_step ? p->batch : 1)};
-  const uint64_t strides[3] = {step_of(p->kv_len > 1, stride[1], p->head_dim, 2), step_of(*head_step, stride[2], p->head_dim, 2),
+  const uint64_t heads = *head_step ? p->kv_heads : 1, batches = *batch_step ? p->batch : 1;
+  const uint64_t dims[4] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(p->kv_len), heads, batches};
+  const uint64_t strides[3] = {step_of(p->kv_len > 1, stride[1], p->head_dim, 2),
+                               step_of(*head_step, stride[2], p->head_dim, 2),
                                step_of(*batch_step, stride[0], p->head_dim, 2)};
   const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
   return op_tensor_map(map, p->type, base, 4, dims, strides, box);
@@ -1030,12 +1054,15 @@ int rows_map(CUtensorMap *map, const struct htpg_attention_params *p, const void
   *head_step = p->q_heads > pack && stride[2] != 0;
   *batch_step = p->batch > 1 && stride[0] != 0;
   const int others = *head_step ? p->q_heads / pack : 1, bytes = type_bytes(type);
-  const uint64_t dims[5] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(pack), static_cast<uint64_t>(p->q_len),
-                            static_cast<uint64_t>(others), static_cast<uint64_t>(*batch_step ? p->batch : 1)};
-  const uint64_t strides[4] = {step_of(pack > 1, stride[2], p->head_dim, bytes), step_of(p->q_len > 1, stride[1], p->head_dim, bytes),
+  const uint64_t dims[5] = {static_cast<uint64_t>(p->head_dim), static_cast<uint64_t>(pack),
+                            static_cast<uint64_t>(p->q_len), static_cast<uint64_t>(others),
+                            static_cast<uint64_t>(*batch_step ? p->batch : 1)};
+  const uint64_t strides[4] = {step_of(pack > 1, stride[2], p->head_dim, bytes),
+                               step_of(p->q_len > 1, stride[1], p->head_dim, bytes),
                                step_of(others > 1, stride[2] * pack, p->head_dim, bytes),
                                step_of(*batch_step, stride[0], p->head_dim, bytes)};
-  const uint32_t box[5] = {static_cast<uint32_t>(128 / bytes), static_cast<uint32_t>(pack), static_cast<uint32_t>(rows / pack), 1, 1};
+  const uint32_t box[5] = {static_cast<uint32_t>(128 / bytes), static_cast<uint32_t>(pack),
+                           static_cast<uint32_t>(rows / pack), 1, 1};
   return op_tensor_map(map, type, base, 5, dims, strides, box);
 }
 
@@ -1048,7 +1075,8 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
   t.pack = (a.group & (a.group - 1)) == 0 && a.group <= 128 && p->q_stride[2] != 0 ? a.group : 1;
   while (1 << t.log_pack < t.pack) ++t.log_pack;
   t.kv_heads = p->kv_heads;
-  const long long row_tiles = (static_cast<long long>(a.q_len) * t.pack + 127) / 128, tiles_kv = row_tiles * (a.group / t.pack);
+  const long long row_tiles = (static_cast<long long>(a.q_len) * t.pack + 127) / 128;
+  const long long tiles_kv = row_tiles * (a.group / t.pack);
   const long long pairs = (tiles_kv + 1) / 2;
   if (pairs > 0x3ffffff) return HTPG_ECAPACITY;
   t.row_tiles = static_cast<int>(row_tiles);
@@ -1075,7 +1103,8 @@ int run_tiles(const struct htpg_attention_params *p, const AttnArgs &a, const Op
     if (qe[i] > 1 && a.os[i] * sizeof(TO) % 32) t.wide = 0;
   CUtensorMap mq, mk, mv;
   int rc;
-  if ((rc = rows_map(&mq, p, a.q, p->type, p->q_stride, t.pack, 128, &t.q_head, &t.q_batch)) || (rc = kv_map(&mk, p, a.k, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
+  if ((rc = rows_map(&mq, p, a.q, p->type, p->q_stride, t.pack, 128, &t.q_head, &t.q_batch)) ||
+      (rc = kv_map(&mk, p, a.k, p->k_stride, KT, &t.k_head, &t.k_batch)) ||
       (rc = kv_map(&mv, p, a.v, p->v_stride, KT, &t.v_head, &t.v_batch)))
     return rc;
   // the output's, where a warp's 32 rows are whole tokens and no two rows are one
@@ -1145,7 +1174,8 @@ int run_few(const struct htpg_attention_params *p, const AttnArgs &a, const OpDe
   long long least = -1;
   for (int s = 1; s <= 64 && (s == 1 || (units * s <= 4 * slots && s * kFewWarps <= chunks)); ++s) {
     const int per = (chunks + s - 1) / s;
-    const long long cost = (units * s + slots - 1) / slots * ((per + kFewWarps - 1) / kFewWarps + (s > 1 ? 6 : 2)) * 4 + (s > 1 ? 2 * s : 0);
+    const long long rounds = (units * s + slots - 1) / slots;
+    const long long cost = rounds * ((per + kFewWarps - 1) / kFewWarps + (s > 1 ? 6 : 2)) * 4 + (s > 1 ? 2 * s : 0);
     if (least < 0 || cost < least) least = cost, f.splits = s;
   }
   f.per = (chunks + f.splits - 1) / f.splits;

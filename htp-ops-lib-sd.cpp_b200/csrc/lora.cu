@@ -482,7 +482,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       }
     }
     if (++at == mine) at = 0, ++group;
-    if (S::kAhead && item + 1 < items && (rb.adapter[z + at * zs] != held || group != held_group)) take(next, z + at * zs, group);
+    if (S::kAhead && item + 1 < items && (rb.adapter[z + at * zs] != held || group != held_group))
+      take(next, z + at * zs, group);
     copy_wait<D - 1>();
     if (rank == 0 && in_place) continue;
     float4 o[2][2];
