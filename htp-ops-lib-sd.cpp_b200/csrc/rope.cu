@@ -180,7 +180,8 @@ __device__ __forceinline__ void store_n(T *p, const float *v) {
 // 8 elements left the pass issue-bound: 4.8 TB/s), and products are packed
 // pairs.  16384 tokens of 36 heads x 128, FP32 to FP16, cold L2: 80 us = 5.7
 // TB/s with two heads per group (one: 92; four: 82; six: 94; 16 elements per
-// lane and part: 80, but 104 against 88 with interleaved pairs).
+// lane and part: 80, but 104 against 88 with interleaved pairs).  FP16 to FP16:
+// 74 us = 4.1 TB/s (one head: 90; four: 86; 16 elements: 84).
 constexpr int kHeads = 2;
 template <typename TI, typename TO, bool HALF, int W>
 __global__ void __launch_bounds__(256) rope_vec_kernel(const __grid_constant__ RopeArgs a, int log_g) {
