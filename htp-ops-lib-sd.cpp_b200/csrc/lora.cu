@@ -303,6 +303,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   using S = UpSmem<T, RK>;
   constexpr int TM = S::TM, PITCH = S::PITCH, PARTS = S::PARTS, D = S::kDepth;
   __shared__ RowBlocks<TM> rb;
+  __shared__ int4 blocks[TM];                     // start, rows, adapter, rank
+  __shared__ long long at_base[TM], at_out[TM];  // of the rows, by place
   __shared__ float undo[TM], shared_sums[kLoraWarps][(RK + 31) / 32 * 32];
   extern __shared__ __align__(16) uint4 smem[];
   __shared__ __align__(16) T ts[PARTS][TM][PITCH];
@@ -314,34 +316,44 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   const int z = blockIdx.z, zs = gridDim.z;
   const int mine = (rb.blocks - z + zs - 1) / zs;  // blocks of this CTA
   const bool in_place = p.base == p.out && p.ldb == p.ldo;
+  if (threadIdx.x < TM && row0 + static_cast<int>(threadIdx.x) < p.m) {
+    const long long row = row0 + rb.row[threadIdx.x];
+    at_base[threadIdx.x] = row * p.ldb;
+    at_out[threadIdx.x] = row * p.ldo;
+  }
+  if (threadIdx.x < rb.blocks)
+    blocks[threadIdx.x] = make_int4(rb.start[threadIdx.x], rb.count[threadIdx.x], rb.adapter[threadIdx.x], rb.rank[rb.start[threadIdx.x]]);
+  __syncthreads();
   // work: column groups of 32 (this warp's), each over the CTA's blocks
   const int c_first = blockIdx.y * n_range + warp * 32, c_end = min(static_cast<int>(blockIdx.y + 1) * n_range, p.n);
   const int groups = c_first < c_end ? (c_end - c_first + kLoraWarps * 32 - 1) / (kLoraWarps * 32) : 0;
   const int items = groups * mine;
   uint4 *ring = smem + warp * (D * 4 * 32) + lane;
-  int f_group = 0, f_block = 0;  // of the next item to fetch
-  auto fetch = [&](int item) {
-    if (item < items && p.base) {
-      const int block = z + f_block * zs, start = rb.start[block], count = rb.count[block];
-      const int c = c_first + f_group * (kLoraWarps * 32) + 8 * t;
-      uint4 *to = ring + item % D * (4 * 32);
+  int f_item = 0, f_block = 0, f_col = c_first + 8 * t;  // of the next item to fetch
+  auto fetch = [&] {
+    if (f_item < items && p.base) {
+      const int4 block = blocks[z + f_block * zs];
+      const bool in = f_col < p.n;
+      const float *src = p.base + (in ? f_col : 0);
+      uint4 *to = ring + f_item % D * (4 * 32);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float *src = p.base + (row0 + rb.row[start + min(g + 8 * i, count - 1)]) * p.ldb;
-        const bool ok = g + 8 * i < count;
-        copy16(to + 2 * i * 32, src + (c < p.n ? c : 0), ok && c < p.n);
-        copy16(to + (2 * i + 1) * 32, src + (c < p.n ? c + 4 : 0), ok && c < p.n);
+        const float *row = src + at_base[block.x + min(g + 8 * i, block.y - 1)];
+        const bool ok = in && g + 8 * i < block.y;
+        copy16(to + 2 * i * 32, row, ok);
+        copy16(to + (2 * i + 1) * 32, row + 4, ok);
       }
-      if (++f_block == mine) f_block = 0, ++f_group;
+      if (++f_block == mine) f_block = 0, f_col += kLoraWarps * 32;
     }
+    ++f_item;
     copy_commit();
   };
   constexpr int V = S::kVec, NVEC = RK / (4 * V);  // vectors of V ranks per lane
   using Vec = std::conditional_t<V == 8, uint4, uint2>;
   // B's vectors for the 32 columns of one group, as they lie
   auto take = [&](Vec (&w)[4][NVEC], int block, int group) {
-    const int rank = rb.rank[rb.start[block]];
-    const T *b = static_cast<const T *>(p.b) + static_cast<long long>(max(rb.adapter[block], 0)) * p.n * p.max_rank;
+    const int rank = blocks[block].w;
+    const T *b = static_cast<const T *>(p.b) + static_cast<long long>(max(blocks[block].z, 0)) * p.n * p.max_rank;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = c_first + group * (kLoraWarps * 32) + 8 * (g >> 1) + 2 * j + (g & 1);
@@ -357,7 +369,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   if (S::kAhead && items > 0) take(next, z, 0);
   grid_dependency_wait();
 #pragma unroll
-  for (int i = 0; i < D - 1; ++i) fetch(i);
+  for (int i = 0; i < D - 1; ++i) fetch();
   {
     // one warp per place, every eighth, a warp's loads of four ranges in flight together
     constexpr int PLACES = TM / kLoraWarps, NV = (RK + 31) / 32;
@@ -456,9 +468,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   __syncthreads();
   int held = -1, held_group = -1, group = 0, at = 0;
   for (int item = 0; item < items; ++item) {
-    fetch(item + D - 1);
-    const int block = z + at * zs, c0 = c_first + group * (kLoraWarps * 32);
-    const int s = rb.adapter[block], start = rb.start[block], count = rb.count[block], rank = rb.rank[start];
+    fetch();
+    const int4 block = blocks[z + at * zs];
+    const int start = block.x, count = block.y, s = block.z, rank = block.w;
+    const int c = c_first + group * (kLoraWarps * 32) + 8 * t;
     if (rank && (s != held || group != held_group)) {
       held = s, held_group = group;
       if (S::kAhead) {
@@ -467,7 +480,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
 #pragma unroll
           for (int k = 0; k < NVEC; ++k) w[j][k] = next[j][k];
       } else {
-        take(w, block, group);
+        take(w, z + at * zs, group);
       }
       if (rank % V) {  // what lies past the rank may be anything
 #pragma unroll
@@ -482,7 +495,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       }
     }
     if (++at == mine) at = 0, ++group;
-    if (S::kAhead && item + 1 < items && (rb.adapter[z + at * zs] != held || group != held_group))
+    if (S::kAhead && item + 1 < items && (blocks[z + at * zs].z != held || group != held_group))
       take(next, z + at * zs, group);
     copy_wait<D - 1>();
     if (rank == 0 && in_place) continue;
@@ -524,11 +537,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
           o[i][h].w = fmaf(acc[2 * h + 1][2 * i + 1], down[i], o[i][h].w);
         }
     }
-    const int c = c0 + 8 * t;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (g + 8 * i >= count || c >= p.n) continue;
-      float *out = p.out + (row0 + rb.row[start + g + 8 * i]) * p.ldo + c;
+      float *out = p.out + at_out[start + g + 8 * i] + c;
       if (p.wide) {
         asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "f"(o[i][0].x), "f"(o[i][0].y),
                      "f"(o[i][0].z), "f"(o[i][0].w), "f"(o[i][1].x), "f"(o[i][1].y), "f"(o[i][1].z), "f"(o[i][1].w)
