@@ -126,21 +126,23 @@ struct DownSmem {
 // the 11 significant bits that TF32 keeps, lo the rest, which TF32 cuts to 11
 // more; A is exact in TF32.  The tensor core's own sums round towards zero, so
 // they are added up outside of it every step.
-// Bound by instructions (16384 x 1536, rank 64: 65 us for 101 MB; the tensor pipe
-// 46 % busy, issue slots 38 %): x is split and A widened in registers.  Both halves
-// of 32 rows in one warp save A's second reading but leave 255 registers and less
-// in flight: 74 us.
-template <typename T, int RK>
+// Bound by the chain of a step (16384 x 1536, rank 64, 101 MB: 67 us in tiles of 32
+// rows, 55 in tiles of 128, where a CTA's set-up and its warps' sums come less
+// often; tensor pipe 46 % busy, issue slots 38 %): x is split and A widened in
+// registers.  Both halves of 32 rows in one warp save A's second reading but leave
+// 255 registers and less in flight: 76 us.
+template <typename T, int RK, int TM>
 __global__ void __launch_bounds__(kLoraThreads, RK >= 64 ? 1 : 2)
     lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range) {
   using S = DownSmem<RK>;
-  constexpr int TM = 32, NT = RK / 8, NS = S::kSteps;
+  constexpr int NT = RK / 8, NS = S::kSteps;
   __shared__ RowBlocks<TM> rb;
   extern __shared__ __align__(16) uint4 smem[];
   grid_dependency_wait();
   grid_dependents_launch();
   const int row0 = blockIdx.x * TM;
-  find_blocks<TM, 32>(rb, p, row0);
+  // 128 rows: a block of 16 rows per warp, and what is left over shared by all
+  find_blocks<TM, TM == 128 ? 16 : 32>(rb, p, row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = blockIdx.y * k_range, k1 = min(k0 + k_range, p.k);
   part += static_cast<long long>(blockIdx.y) * p.m * p.max_rank;
@@ -556,15 +558,32 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
 
 template <typename T, int RK>
 int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
-  // Down: ranges of K until every SM has a tile (multiples of 128, none shorter
-  // than a step per warp: 1000 mixed rows 21.5 us in all; multiples of 256 22.5;
-  // two CTAs per SM 23.9), then a tile's blocks side by side.
   using U = UpSmem<T, RK>;
   using D = DownSmem<RK>;
-  const int tiles = (p.m + 31) / 32, parts = (p.k + 127) / 128;
-  const int ranges = std::max(1, std::min(parts / 2, d.sms / tiles));
-  const int k_range = (parts + ranges - 1) / ranges * 128;
-  const int k_ranges = (p.k + k_range - 1) / k_range;
+  // Down: ranges of K until every SM has a tile (multiples of 128, none shorter
+  // than a step per warp: 1000 mixed rows 21.5 us in all; multiples of 256 22.5;
+  // two CTAs per SM 23.9), then a tile's blocks side by side.  Tiles of 32 or, up
+  // to rank 64, 128 rows, whichever takes fewer rounds of (rows x elements + a CTA's
+  // set-up, about as long as 32 rows x 1024 elements): 16384 x 1536 x 6144, rank 64:
+  // 226 us in all with 32, 216 with 128; mixed, rank 16: 269, 247; rank 128: 210, 215.
+  struct Plan {
+    int tiles, k_range, k_ranges;
+    long long cost;
+  };
+  auto plan = [&](int rows) {
+    Plan r;
+    r.tiles = (p.m + rows - 1) / rows;
+    const int parts = (p.k + 127) / 128, ranges = std::max(1, std::min(parts / 2, d.sms / r.tiles));
+    r.k_range = (parts + ranges - 1) / ranges * 128;
+    r.k_ranges = (p.k + r.k_range - 1) / r.k_range;
+    const long long rounds = (static_cast<long long>(r.tiles) * r.k_ranges + d.sms - 1) / d.sms;
+    r.cost = rounds * (rows / 32 * static_cast<long long>(std::min(r.k_range, p.k)) + 1024);
+    return r;
+  };
+  const Plan small = plan(32), large = plan(128);
+  const bool wide_tiles = RK <= 64 && large.cost < small.cost;
+  const Plan down_plan = wide_tiles ? large : small;
+  const int tiles = down_plan.tiles, k_range = down_plan.k_range, k_ranges = down_plan.k_ranges;
   const int z_down = std::max(1, std::min({8, p.adapters, p.m, d.sms / (tiles * k_ranges)}));
   // Up: the column ranges whose rounds of CTAs (two per SM) do least, a CTA's
   // set-up counted as two steps of 256 columns; then blocks of rows side by side.
@@ -585,7 +604,7 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   const int rc = op_scratch(st, static_cast<size_t>(k_ranges) * p.m * p.max_rank * sizeof(float), &counters, &scratch);
   if (rc) return rc;
   float *part = reinterpret_cast<float *>(scratch);
-  auto *down = lora_down_kernel<T, RK>;
+  auto *down = wide_tiles ? lora_down_kernel<T, RK, RK <= 64 ? 128 : 32> : lora_down_kernel<T, RK, 32>;
   auto *up = lora_up_kernel<T, RK>;
   cudaError_t e = cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, D::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, U::kBytes);
