@@ -278,7 +278,9 @@ struct UpSmem {
   static constexpr int PITCH = RK == 64 ? 96 : RK == 128 ? 160 : RK;
   static constexpr int kVec = RK >= 32 ? 8 : 4;  // ranks a lane holds together
   static constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
-  static constexpr int kDepth = 4;  // blocks of base in flight per warp
+  // Blocks of base in flight per warp, less one: more leave less L1 for the rest
+  // (16384 x 1536 x 6144, rank 64: two 214 us, three 208, four 217, five 265).
+  static constexpr int kDepth = 3;
   // The next item's part of B is read ahead, the first before t (one row, 4096 x
   // 14336: 8.6 -> 8.0 us; 16384 mixed rows of rank 16: 300 -> 283); above rank 32
   // the registers do not reach.
@@ -501,55 +503,52 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       take(next, z + at * zs, group);
     copy_wait<D - 1>();
     if (rank == 0 && in_place) continue;
-    float4 o[2][2];
+    // base joins after the products: 16 registers fewer next to B (rank 128: 210 -> 190 us)
+    float acc[4][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+    // places past the block's rows: those of other blocks, whose results are not stored
+    const int r0 = min(start + g, TM - 1), r1 = min(start + g + 8, TM - 1);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        o[i][h] = p.base ? *reinterpret_cast<const float4 *>(ring + (item % D * 4 + 2 * i + h) * 32) : make_float4(0, 0, 0, 0);
-    if (rank) {
-      float acc[4][4];
+    for (int k = 0; k < NVEC; ++k) {
+      if (4 * V * k >= rank) break;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-      // places past the block's rows: those of other blocks, whose results are not stored
-      const int r0 = min(start + g, TM - 1), r1 = min(start + g + 8, TM - 1);
+      for (int q = PARTS - 1; q >= 0; --q) {
+        const Vec v0 = *reinterpret_cast<const Vec *>(&ts[q][r0][4 * V * k + V * t]);
+        const Vec v1 = *reinterpret_cast<const Vec *>(&ts[q][r1][4 * V * k + V * t]);
 #pragma unroll
-      for (int k = 0; k < NVEC; ++k) {
-        if (4 * V * k >= rank) break;
+        for (int e = 0; e < V / 4; ++e) {
+          const uint32_t a[4] = {word(v0, 2 * e), word(v1, 2 * e), word(v0, 2 * e + 1), word(v1, 2 * e + 1)};
 #pragma unroll
-        for (int q = PARTS - 1; q >= 0; --q) {
-          const Vec v0 = *reinterpret_cast<const Vec *>(&ts[q][r0][4 * V * k + V * t]);
-          const Vec v1 = *reinterpret_cast<const Vec *>(&ts[q][r1][4 * V * k + V * t]);
-#pragma unroll
-          for (int e = 0; e < V / 4; ++e) {
-            const uint32_t a[4] = {word(v0, 2 * e), word(v1, 2 * e), word(v0, 2 * e + 1), word(v1, 2 * e + 1)};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma_16<T>(acc[j], a, word(w[j][k], 2 * e), word(w[j][k], 2 * e + 1));
-          }
+          for (int j = 0; j < 4; ++j) mma_16<T>(acc[j], a, word(w[j][k], 2 * e), word(w[j][k], 2 * e + 1));
         }
       }
-      const float down[2] = {undo[r0], undo[r1]};
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          o[i][h].x = fmaf(acc[2 * h][2 * i], down[i], o[i][h].x);
-          o[i][h].y = fmaf(acc[2 * h][2 * i + 1], down[i], o[i][h].y);
-          o[i][h].z = fmaf(acc[2 * h + 1][2 * i], down[i], o[i][h].z);
-          o[i][h].w = fmaf(acc[2 * h + 1][2 * i + 1], down[i], o[i][h].w);
-        }
     }
+    const float down[2] = {undo[r0], undo[r1]};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (g + 8 * i >= count || c >= p.n) continue;
+      float4 o[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float *x = acc[2 * h], *y = acc[2 * h + 1];
+        o[h] = make_float4(0, 0, 0, 0);
+        if (p.base) o[h] = *reinterpret_cast<const float4 *>(ring + (item % D * 4 + 2 * i + h) * 32);
+        if (rank) {
+          o[h].x = fmaf(x[2 * i], down[i], o[h].x);
+          o[h].y = fmaf(x[2 * i + 1], down[i], o[h].y);
+          o[h].z = fmaf(y[2 * i], down[i], o[h].z);
+          o[h].w = fmaf(y[2 * i + 1], down[i], o[h].w);
+        }
+      }
       float *out = p.out + at_out[start + g + 8 * i] + c;
       if (p.wide) {
-        asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "f"(o[i][0].x), "f"(o[i][0].y),
-                     "f"(o[i][0].z), "f"(o[i][0].w), "f"(o[i][1].x), "f"(o[i][1].y), "f"(o[i][1].z), "f"(o[i][1].w)
+        asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "f"(o[0].x),
+                     "f"(o[0].y), "f"(o[0].z), "f"(o[0].w), "f"(o[1].x), "f"(o[1].y), "f"(o[1].z), "f"(o[1].w)
                      : "memory");
       } else {
-        __stcs(reinterpret_cast<float4 *>(out), o[i][0]);
-        __stcs(reinterpret_cast<float4 *>(out + 4), o[i][1]);
+        __stcs(reinterpret_cast<float4 *>(out), o[0]);
+        __stcs(reinterpret_cast<float4 *>(out + 4), o[1]);
       }
     }
   }
