@@ -127,8 +127,8 @@ struct DownSmem {
 // more; A is exact in TF32.  The tensor core's own sums round towards zero, so
 // they are added up outside of it every step.
 // Bound by the chain of a step (16384 x 1536, rank 64, 101 MB: 67 us in tiles of 32
-// rows, 55 in tiles of 128, where a CTA's set-up and its warps' sums come less
-// often; tensor pipe 46 % busy, issue slots 38 %): x is split and A widened in
+// rows, 57 in tiles of 128, where a CTA's set-up and its warps' sums come less
+// often; tensor pipe 57 % busy, issue slots 43 %): x is split and A widened in
 // registers.  Both halves of 32 rows in one warp save A's second reading but leave
 // 255 registers and less in flight: 76 us.
 template <typename T, int RK, int TM>
@@ -299,8 +299,9 @@ struct UpSmem {
 // pieces and a row's 32 outputs are one 128-byte line of one store.  Each warp keeps
 // kDepth blocks (16 rows x 32 columns) of base in flight in a ring of its own, read
 // back by the lanes that copied them.
-// Bound by HBM through base and out: 16384 rows x 6144, rank 64: 165 us for 805 MB
-// (4.9 TB/s); few rows by the chain ids -> t -> out (one row, both passes: 8 us).
+// Many rows: bound by L1 and the chain of an item, then HBM (16384 rows x 6144, rank
+// 64: 169 us for 805 MB, L1 78 % busy; both passes 208 us in a sequence); few rows
+// by the chain ids -> t -> out (one row, both passes: 8 us).
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, 2)
     lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range) {
@@ -584,14 +585,18 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   const Plan down_plan = wide_tiles ? large : small;
   const int tiles = down_plan.tiles, k_range = down_plan.k_range, k_ranges = down_plan.k_ranges;
   const int z_down = std::max(1, std::min({8, p.adapters, p.m, d.sms / (tiles * k_ranges)}));
-  // Up: the column ranges whose rounds of CTAs (two per SM) do least, a CTA's
-  // set-up counted as two steps of 256 columns; then blocks of rows side by side.
+  // Up: the column ranges that take least, in sixths of a step of 256 columns: two
+  // CTAs of one SM take 5/3 of the time of one, and a CTA's set-up as long as two
+  // steps; then blocks of rows side by side.  Against whole rounds of two per SM,
+  // 12867 rows of 1152 x 4608, in all: rank 32 176 -> 158 us, rank 64 173 -> 160
+  // (BF16) and 156 -> 162 (FP16), rank 16 114 -> 123.
   const int up_tiles = (p.m + U::TM - 1) / U::TM, n_steps = (p.n + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
   int n_range = n_steps;
   long long least = -1;
   for (int per = 1; per <= n_steps; ++per) {
     const long long ctas = static_cast<long long>(up_tiles) * ((n_steps + per - 1) / per);
-    const long long cost = (ctas + 2 * d.sms - 1) / (2 * d.sms) * (per + 2);
+    const long long each = (ctas + d.sms - 1) / d.sms;  // per SM
+    const long long cost = (each == 1 ? 6 : 5 * each) * per + 12 * each;
     if (least < 0 || cost <= least) least = cost, n_range = per;
   }
   n_range *= kLoraWarps * 32;
