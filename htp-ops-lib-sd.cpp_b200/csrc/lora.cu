@@ -131,15 +131,17 @@ struct DownSmem {
 // often; tensor pipe 57 % busy, issue slots 43 %): x is split and A widened in
 // registers.  Both halves of 32 rows in one warp save A's second reading but leave
 // 255 registers and less in flight: 76 us.
+// One CTA per SM: registers for all of a step's loads (rank 32: 166 instead of 128,
+// 12867 x 1152 x 4608 145 -> 131 us in all).
 template <typename T, int RK, int TM>
-__global__ void __launch_bounds__(kLoraThreads, RK >= 64 ? 1 : 2)
-    lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range) {
+__global__ void __launch_bounds__(kLoraThreads, 1)
+    lora_down_kernel(const __grid_constant__ LoraArgs p, float *part, int k_range, int early) {
   using S = DownSmem<RK>;
   constexpr int NT = RK / 8, NS = S::kSteps;
   __shared__ RowBlocks<TM> rb;
   extern __shared__ __align__(16) uint4 smem[];
   grid_dependency_wait();
-  grid_dependents_launch();
+  if (early) grid_dependents_launch();
   const int row0 = blockIdx.x * TM;
   // 128 rows: a block of 16 rows per warp, and what is left over shared by all
   find_blocks<TM, TM == 128 ? 16 : 32>(rb, p, row0);
@@ -588,8 +590,8 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   // Up: the column ranges that take least, in sixths of a step of 256 columns: two
   // CTAs of one SM take 5/3 of the time of one, and a CTA's set-up as long as two
   // steps; then blocks of rows side by side.  Against whole rounds of two per SM,
-  // 12867 rows of 1152 x 4608, in all: rank 32 176 -> 158 us, rank 64 173 -> 160
-  // (BF16) and 156 -> 162 (FP16), rank 16 114 -> 123.
+  // 12867 rows of 1152 x 4608, in all: rank 64 173 -> 160 us (BF16) and 156 -> 162 (FP16),
+  // rank 16 114 -> 123, rank 32 176 -> 158 (131 as it is now).
   const int up_tiles = (p.m + U::TM - 1) / U::TM, n_steps = (p.n + kLoraWarps * 32 - 1) / (kLoraWarps * 32);
   int n_range = n_steps;
   long long least = -1;
@@ -602,6 +604,10 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   n_range *= kLoraWarps * 32;
   const int n_ranges = (p.n + n_range - 1) / n_range;
   const int z_up = std::max(1, std::min({8, p.adapters, p.m, 2 * d.sms / (up_tiles * n_ranges)}));
+  // The second pass is let in early, to find its blocks meanwhile, for few rows only:
+  // with many its CTAs crowd on the SMs that are free then (rank 32, both passes:
+  // 1000 rows 16.5 us early, 18.9 late; 4096 x 1536 x 4608 63.6 and 50.3).
+  const int early = p.m <= 2048;
   auto lock = op_lock();
   uint32_t *counters;
   uint8_t *scratch;
@@ -612,7 +618,7 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   auto *up = lora_up_kernel<T, RK>;
   cudaError_t e = cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, D::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, U::kBytes);
-  if (e == cudaSuccess) e = op_launch(down, dim3(tiles, k_ranges, z_down), kLoraThreads, D::kBytes, st, p, part, k_range);
+  if (e == cudaSuccess) e = op_launch(down, dim3(tiles, k_ranges, z_down), kLoraThreads, D::kBytes, st, p, part, k_range, early);
   if (e == cudaSuccess) e = op_launch(up, dim3(up_tiles, n_ranges, z_up), kLoraThreads, U::kBytes, st, p, part, k_ranges, n_range);
   return op_result(e);
 }
