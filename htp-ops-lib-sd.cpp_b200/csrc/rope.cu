@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_row_kernel(RopeArgs a) {
     if (rot) {
       const long long pos = a.positions ? a.positions[token] : i;
       const bool ok = pos >= 0 && pos < a.table_rows;
-      const float2 *cs = a.table + (ok ? pos : 0) * (rot / 2);
-      for (int j = lane; j < rot / 2; j += 32) {
+      const float2 *cs = a.table + pos * (rot / 2);
+      for (int j = lane; ok && j < rot / 2; j += 32) {  // outside: the table may have no row at all
         const int d0 = a.half ? j : 2 * j, d1 = a.half ? j + rot / 2 : 2 * j + 1;
         const float2 w = cs[j];
         const float u = row[d0], v = row[d1];

@@ -201,3 +201,23 @@ def test_table(gpu, rows, rot, kw):
     got = table_of(rows, rot, gpu, **kw).cpu().double()
     # angles up to 2^17 in FP64 from a power and a product good to 2^-51: 2^-34; the store rounds by 2^-25 (values < 2)
     assert float((got - table_fp64(rows, rot, **kw)).abs().max()) <= 2.0**-24
+
+
+@pytest.mark.parametrize("src", [F32, F16])
+@pytest.mark.parametrize("d,rot,half", [(33, 30, 0), (33, 30, 1), (7, 2, 0), (510, 254, 1), (64, 64, 1)])
+def test_positions_outside_the_table_at_any_head_dim(gpu, d, rot, half, src):
+    """As above at sizes without vectors, and with a table that has no row."""
+    x = torch.ones(2, 3, 2, d, device=gpu).to(src)
+    table = table_of(16, rot, gpu)
+    pos = torch.tensor([[3, -1, 16], [-2**31, 2**31 - 1, 15]], dtype=torch.int32, device=gpu)
+    outs = [torch.zeros_like(x) for _ in range(3)]
+    prm = htpg.rope_params(x, x, x, *outs, rot, half, 16)
+    assert htpg.qkv_rope(prm, *outs, x, x, x, table=table, positions=pos) == 0
+    inside = (pos >= 0) & (pos < 16)
+    for o in outs[:2]:
+        close(o[inside][:, None], *(y[inside][:, None] for y in rotated(x, table, pos.clamp(0, 15), rot, half, None)))
+        assert bool(o[~inside].isnan().all())
+    assert torch.equal(outs[2], x)
+    prm = htpg.rope_params(x, x, x, *outs, rot, half, 0)
+    assert htpg.qkv_rope(prm, *outs, x, x, x, table=table, positions=pos) == 0
+    assert all(bool(o.isnan().all()) for o in outs[:2]) and torch.equal(outs[2], x)
