@@ -554,9 +554,12 @@ def cross_attention(prm: AttentionParams, out, q, k, v, kv_lens=None, key_bias=N
 
 def lora_params(out, base, x, a, b) -> LoraParams:
     """Parameters of lora_run: x [m][k], out and base [m][n] FP32, a [adapters][max_rank][k], b [adapters][n][max_rank]."""
+    import torch
     if a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.dtype != b.dtype or a.shape[2] != x.shape[1] or \
             b.shape[1] != out.shape[1] or x.shape[0] != out.shape[0] or (base is not None and base.shape != out.shape):
         raise ValueError("x, a, b, base and out do not fit together")
+    if any(t is not None and t.dtype != torch.float32 for t in (x, base, out)):
+        raise ValueError("x, base and out are FP32")
     if not (a.is_contiguous() and b.is_contiguous()):
         raise ValueError("a and b are dense")
     if any(t is not None and t.stride(1) != 1 for t in (x, base, out)):
