@@ -564,6 +564,8 @@ def lora_params(out, base, x, a, b) -> LoraParams:
         raise ValueError("a and b are dense")
     if any(t is not None and t.stride(1) != 1 for t in (x, base, out)):
         raise ValueError("rows of x, base and out are contiguous")
+    if any(t is not None and t.shape[0] > 1 and t.stride(0) < t.shape[1] for t in (x, base, out)):
+        raise ValueError("rows of x, base and out have memory of their own (an expanded one needs a copy)")
     return LoraParams(type_of(a), x.shape[0], x.shape[1], out.shape[1], a.shape[0], a.shape[1], x.stride(0),
                       base.stride(0) if base is not None else 0, out.stride(0))
 

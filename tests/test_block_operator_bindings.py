@@ -23,3 +23,19 @@ def test_lora_activations_are_fp32(name, dtype):
     t[name] = t[name].to(dtype)
     with pytest.raises(ValueError, match="FP32"):
         htpg.lora_params(**t)
+
+
+@pytest.mark.parametrize("name", ["out", "base", "x"])
+def test_lora_rows_that_are_one_row_are_refused(name):
+    """A row stride of 0 means dense to the library: m rows would be read where there is one."""
+    t = lora()
+    t[name] = t[name][:1].expand(5, -1)
+    with pytest.raises(ValueError, match="own"):
+        htpg.lora_params(**t)
+    t = lora()
+    t[name] = t[name].as_strided(t[name].shape, (8, 1))  # rows that overlap
+    with pytest.raises(ValueError, match="own"):
+        htpg.lora_params(**t)
+    one = lora(m=1)  # of a single row the stride is not looked at
+    one[name] = one[name].as_strided(one[name].shape, (0, 1))
+    assert htpg.lora_params(**one).m == 1
