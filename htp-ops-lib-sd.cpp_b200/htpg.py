@@ -449,7 +449,9 @@ def aux_params_bytes(prm: dict, eps: float = 1e-6, output=(-1, 0), input_=(-1, 0
 # ------------------------------------------------------------------ transformer block operators
 # Per-head norm and rotation, cross attention and low-rank adapters.  Each call
 # takes a parameter block (sizes, types, strides) built once from its tensors
-# and the tensors' addresses of this call; it returns the library's code.
+# and the tensors' addresses of this call; it returns the library's code.  The
+# tensors are those of the block, or have their types, shapes and strides; the
+# arrays that the block does not describe are looked at in the call (ValueError).
 class RopeScaling(ctypes.Structure):
     """struct htpg_rope_scaling."""
     _fields_ = [("scaling", ctypes.c_int32), ("original_rows", ctypes.c_int32), ("base", ctypes.c_double),
@@ -498,11 +500,54 @@ def _strides(t):
     return t.stride()[:3]
 
 
+def _on_device(t) -> bool:
+    """Whether kernels can read t, a tensor outside of device memory: pinned host memory."""
+    return t.is_pinned()
+
+
+def _dptr(t) -> int | None:
+    """ptr() of a tensor that kernels can read."""
+    if t is None:
+        return None
+    if t.is_cuda or _on_device(t):
+        return t.data_ptr()
+    raise ValueError("a tensor in pageable host memory")
+
+
+def _array(t, name: str, dtype, n: int) -> int | None:
+    """Address of an array of a call: dense, at least n elements of one type (the library sees the address alone)."""
+    if t is None:
+        return None
+    if t.dtype is dtype and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr() if t.is_cuda else _dptr(t)
+    raise ValueError(f"{name}: expected a dense {dtype} array of {n} elements or more, got {tuple(t.shape)}, strides "
+                     f"{t.stride()}, {t.dtype}")
+
+
+def _bias(t, prm) -> int | None:
+    """Address of a key bias: FP32, prm.batch rows of prm.kv_len elements, prm.bias_stride apart."""
+    if t is None:
+        return None
+    import torch
+    step, keys, shape = prm.bias_stride, prm.kv_len, t.shape
+    reach = (prm.batch - 1) * step + keys  # elements from the first to the last that are read
+    if t.dtype is torch.float32 and step >= 0 and shape[-1] >= keys:
+        inside = t.numel()
+        if not t.is_contiguous():
+            inside = 1 + sum((n - 1) * s for n, s in zip(shape, t.stride())) if t.stride(-1) == 1 else 0
+        if inside >= reach:
+            return _dptr(t)
+    raise ValueError(f"key_bias: expected {prm.batch} FP32 rows of {keys}, {step} elements apart, got {tuple(shape)}, "
+                     f"strides {t.stride()}, {t.dtype}")
+
+
 def rope_table(table, rot_dim: int, scaling: int = ROPE_PLAIN, base: float = 10000.0, factor: float = 1.0,
                original_rows: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0, stream=None) -> int:
     """Fill table [rows][rot_dim / 2][2] (FP32) with cosines and sines of rotary positions."""
+    import torch
     s = RopeScaling(scaling, original_rows, base, factor, beta_fast, beta_slow)
-    return lib().htpg_rope_table(ptr(table), table.shape[0], rot_dim, ctypes.byref(s), stream_ptr(stream))
+    at = _array(table, "table", torch.float32, table.shape[0] * rot_dim)
+    return lib().htpg_rope_table(at, table.shape[0], rot_dim, ctypes.byref(s), stream_ptr(stream))
 
 
 def rope_params(q, k, v, q_out, k_out, v_out, rot_dim: int, layout: int, table_rows: int,
@@ -529,8 +574,13 @@ def rope_params(q, k, v, q_out, k_out, v_out, rot_dim: int, layout: int, table_r
 
 def qkv_rope(prm: RopeParams, q_out, k_out, v_out, q, k, v, q_weight=None, k_weight=None, table=None,
              positions=None, stream=None) -> int:
-    return lib().htpg_qkv_rope(ctypes.byref(prm), ptr(q_out), ptr(k_out), ptr(v_out), ptr(q), ptr(k), ptr(v),
-                               ptr(q_weight), ptr(k_weight), ptr(table), ptr(positions), stream_ptr(stream))
+    """Weights FP32 [dim], table FP32 [table_rows][rot_dim / 2][2], positions int32 [batch][seq]: dense."""
+    import torch
+    f32, dim = torch.float32, prm.head_dim
+    return lib().htpg_qkv_rope(ctypes.byref(prm), _dptr(q_out), _dptr(k_out), _dptr(v_out), _dptr(q), _dptr(k), _dptr(v),
+                               _array(q_weight, "q_weight", f32, dim), _array(k_weight, "k_weight", f32, dim),
+                               _array(table, "table", f32, prm.table_rows * prm.rot_dim),
+                               _array(positions, "positions", torch.int32, prm.batch * prm.seq), stream_ptr(stream))
 
 
 def attention_params(out, q, k, v, scale: float, bias_stride: int | None = None) -> AttentionParams:
@@ -548,8 +598,11 @@ def attention_params(out, q, k, v, scale: float, bias_stride: int | None = None)
 
 
 def cross_attention(prm: AttentionParams, out, q, k, v, kv_lens=None, key_bias=None, stream=None) -> int:
-    return lib().htpg_cross_attention(ctypes.byref(prm), ptr(out), ptr(q), ptr(k), ptr(v), ptr(kv_lens),
-                                      ptr(key_bias), stream_ptr(stream))
+    """kv_lens: int32 [batch], dense; key_bias: FP32, rows of kv_len elements prm.bias_stride apart."""
+    import torch
+    return lib().htpg_cross_attention(ctypes.byref(prm), _dptr(out), _dptr(q), _dptr(k), _dptr(v),
+                                      _array(kv_lens, "kv_lens", torch.int32, prm.batch), _bias(key_bias, prm),
+                                      stream_ptr(stream))
 
 
 def lora_params(out, base, x, a, b) -> LoraParams:
@@ -571,5 +624,9 @@ def lora_params(out, base, x, a, b) -> LoraParams:
 
 
 def lora_run(prm: LoraParams, out, base, x, row_adapter, a, b, ranks, scales, stream=None) -> int:
-    return lib().htpg_lora_run(ctypes.byref(prm), ptr(out), ptr(base), ptr(x), ptr(row_adapter), ptr(a), ptr(b),
-                               ptr(ranks), ptr(scales), stream_ptr(stream))
+    """row_adapter int32 [m], ranks int32 and scales FP32 [adapters]: dense."""
+    import torch
+    return lib().htpg_lora_run(ctypes.byref(prm), _dptr(out), _dptr(base), _dptr(x),
+                               _array(row_adapter, "row_adapter", torch.int32, prm.m), _dptr(a), _dptr(b),
+                               _array(ranks, "ranks", torch.int32, prm.adapters),
+                               _array(scales, "scales", torch.float32, prm.adapters), stream_ptr(stream))
