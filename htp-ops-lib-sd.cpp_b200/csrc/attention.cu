@@ -153,6 +153,13 @@ __device__ __forceinline__ TileItem tile_item(const TileArgs &t, int item, const
   return r;
 }
 
+// A key's bias in units of log2.  The lowest finite ones stay finite (-inf would
+// take their keys out); NaN stays NaN.
+__device__ __forceinline__ float bias_log2(float add) {
+  add *= kLog2e;
+  return add == -INFINITY ? -3.402823466e38f : add;
+}
+
 __device__ __forceinline__ void store32(void *p, const uint32_t (&v)[8], bool wide) {
   if (wide) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -454,12 +461,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int k0 = (it.j0 + j) * KT, keys = min(KT, it.n - k0);
         bool dead = r < KT && r >= keys;
         if (bias) {
-          // one key per thread: in units of log2, the lowest finite bias kept
-          // finite; two buffers, taken in turn over all steps (a thread may be
-          // one barrier ahead of the slowest reader), so one barrier a step is enough
+          // one key per thread; two buffers, taken in turn over all steps (a thread
+          // may be one barrier ahead of the slowest reader), so one barrier a step is
+          // enough
           float add = r < keys ? ld_dep(bias + k0 + r) : -INFINITY;
           dead = r < KT && add == -INFINITY;
-          if (!dead) add = fmaxf(add * kLog2e, -3.402823466e38f);
+          if (!dead) add = bias_log2(add);
           if (r < KT) bias_s[(seen & 1) * KT + r] = add;
           named_bar_sync(1 + w, 128);
         }
@@ -865,7 +872,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
           float add = key < n ? 0.0f : -INFINITY;
           if (bias && key < n) {
             add = ld_dep(bias + key);
-            if (add != -INFINITY) add = fmaxf(add * kLog2e, -3.402823466e38f);  // the lowest finite bias stays finite
+            if (add != -INFINITY) add = bias_log2(add);
           }
           s[h][e] = add == -INFINITY ? -INFINITY : fmaf(s[h][e], c, add);
           s[h][2 + e] = add == -INFINITY ? -INFINITY : fmaf(s[h][2 + e], c, add);

@@ -273,7 +273,8 @@ int htpg_qkv_rope(const struct htpg_rope_params *p, void *q_out, void *k_out, vo
  * h' = h / (q_heads / kv_heads).  Only keys j < kv_lens[b] (clamped to [0,
  * kv_len]; NULL: kv_len) whose bias is not -inf take part: whatever K and V
  * hold at the others, infinities and NaN included, changes nothing.  A row
- * with no such key is zero.  key_bias: FP32 [batch][kv_len] (row stride
+ * with no such key is zero.  A NaN bias of a key j < kv_lens[b] makes the batch's
+ * rows NaN.  key_bias: FP32 [batch][kv_len] (row stride
  * bias_stride elements, 0 shares one row), or NULL.
  *
  * q, out: [batch][q_len][q_heads][head_dim]; k, v: [batch][kv_len][kv_heads]
