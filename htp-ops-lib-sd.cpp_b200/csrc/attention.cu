@@ -455,6 +455,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool mine = token < t.a.q_len;
       const float *bias = t.a.bias ? t.a.bias + it.b * t.a.bias_stride : nullptr;
       const float unit = bias ? 1.0f : c;  // of the scores in s[], in log2
+      // top: what weights are relative to, the held maximum less kShift.  It is kept as
+      // rounded, so that weights, sums and key ranges agree where scores are so large
+      // that FP32 cannot take kShift off exactly, and is compared by differences
+      // (exact there), so that weights stay within 2^(kLazy + kShift).
       float top = -INFINITY, sum = 0.0f;
       if (w == 1 && nt) named_bar_arrive(3 + quad, 64);  // tile 0 begins
       for (int j = 0; j < nt; ++j, used += 2) {
@@ -504,11 +508,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int x = 0; x < KT / 2; ++x)
             most4[x % 4] = fmaxf(most4[x % 4], fmaxf(s[x / 16][x % 16].x, s[x / 16][x % 16].y));
           const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3])) * unit;
-          const bool raise = most > top + kLazy || (top == -INFINITY && most > -INFINITY);
+          const bool raise = most - top > kLazy + kShift;  // from -inf too; NaN where both are -inf: no
           if (__any_sync(0xffffffffu, raise)) {
-            const float keep = raise ? ex2_approx(top - most) : 1.0f;
+            const float to = most - kShift, keep = raise ? ex2_approx(top - to) : 1.0f;
             if (raise) {
-              top = most;
+              top = to;
               sum *= keep;
             }
             if (j > 0) {
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // they fall into step, and the exponential unit idles in between).
         if (it.two) named_bar_sync(3 + 4 * w + quad, 64);
         if (ok) {
-          const float from = top == -INFINITY ? 0.0f : top - kShift;
+          const float from = top == -INFINITY ? 0.0f : top;
           const float2 zero2 = make_float2(0.0f, 0.0f);
           float2 sum4[4] = {make_float2(sum, 0.0f), zero2, zero2, zero2};
 #pragma unroll
@@ -890,6 +894,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
       float most = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      most -= kShift;  // as rounded: weights, sums and ranges agree where it is not exact
       const bool up = most > top[i];
       keep[i] = up ? ex2_approx(top[i] - most) : 1.0f;
       if (up) top[i] = most;
@@ -903,7 +908,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attn_few_kernel(const __gri
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float from = top[i] == -INFINITY ? 0.0f : top[i] - kShift;
+      const float from = top[i] == -INFINITY ? 0.0f : top[i];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float p0 = ex2_approx(s[h][2 * i] - from), p1 = ex2_approx(s[h][2 * i + 1] - from);

@@ -1,4 +1,5 @@
-"""Key biases at the ends of their range (htpg_cross_attention)."""
+"""Key biases at the ends of their range (htpg_cross_attention): NaN, and values
+so large that FP32 scores are whole numbers and coarser."""
 import pytest
 import torch
 
@@ -31,3 +32,22 @@ def test_nan_bias_of_a_key_that_takes_part_is_nan(gpu, n, m, d, src, dst):
     assert bool(out[[1, 2, 4]].isnan().all())
     ok = [0, 3, 5]
     close(out[ok], q[ok], k[ok], v[ok], 0.125, lens[ok], torch.nan_to_num(bias[ok], nan=-INF))
+
+
+@pytest.mark.parametrize("src,dst", TYPES)
+@pytest.mark.parametrize("n,m", [(1, 640), (16, 640), (200, 640), (130, 4096)])
+@pytest.mark.parametrize("far", [1e4, 1e6, 1.3e7, 2e7, 3e7, 5e7, 1e8, 1e9, 1e30])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_far_biases_keep_weights_in_range(gpu, n, m, src, dst, far, sign):
+    """Every key's bias is far from zero, and rises along the keys by what its FP32 value can still show (at least 4)."""
+    q, k, v, g = inputs(gpu, 1, n, m, 2, 2, 64, src)
+    step = max(4.0, far * 2.0**-23)
+    bias = (sign * far + step * torch.floor(torch.arange(m, device=gpu) / 64 * 2) / 2)[None].float()
+    out, scale = call(q, k, v, dst, bias=bias)
+    assert bool(out.isfinite().all())
+    low, high = (getattr(v.double(), f)(1, keepdim=True) for f in ("amin", "amax"))  # an average of values
+    slack = 2.0**-7 * v.abs().max().double()
+    assert bool((out >= low - slack).all()) and bool((out <= high + slack).all())
+    # keys in order of their bias: what is 60 below the last keys' has no weight
+    seen = bias[0] >= bias[0, -1] - 60 - far * 2.0**-20
+    close(out, q, k[:, seen], v[:, seen], scale, None, bias[:, seen])
