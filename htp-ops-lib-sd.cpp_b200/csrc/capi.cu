@@ -1177,13 +1177,19 @@ int op_tensor_map(CUtensorMap *map, int type, const void *base, int rank, const 
   cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
-  const CUresult r = g_encode(map,
-                              type == HTPG_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                              : type == HTPG_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                              rank, const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return g_encode(map,
+                    type == HTPG_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                    : type == HTPG_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                    rank, const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a host thread's first CUDA work: the device's context is not yet its own
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     t_last_cuda_error = "cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")";
     return HTPG_ELAUNCH;
