@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <tuple>
@@ -51,8 +52,27 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
 struct Workspace {
   void *base = nullptr;
   size_t bytes = 0;
-  bool captured = false;  // ows: a captured graph may refer to the block
 };
+
+// A block of the block operators' scratch (op_scratch): a stream's, or one that
+// a captured graph holds for the calls of one of its streams.
+struct OpBlock {
+  uint8_t *base = nullptr;
+  size_t bytes = 0;
+  unsigned long long capture = 0;  // the graph's: id of its capture, and the stream in it
+  const void *owner = nullptr;
+  std::atomic<bool> held{true};  // false: nothing runs with it or ever will, it may be reused or freed
+  bool dead = false;             // let go of while work with it may still run: only freed
+};
+
+struct OpStream {
+  cudaStream_t handle = nullptr;
+  OpBlock *block = nullptr;
+  unsigned long long used = 0;  // when last
+};
+// Streams with a block; one more takes the place of the one that called longest
+// ago (streams that were destroyed cannot be told from idle ones).
+constexpr size_t kOpStreams = 128;
 
 struct Device {
   bool ready = false;
@@ -61,7 +81,10 @@ struct Device {
   uint32_t *watchdog = nullptr;
   std::map<cudaStream_t, Workspace> ws;
   std::map<cudaStream_t, Workspace> qws;  // opcodes 2-4: counters | partials | FP16 operands
-  std::map<cudaStream_t, Workspace> ows;  // block operators: counters | partials
+  std::map<unsigned long long, OpStream> ows;  // block operators, by stream id: counters | partials
+  std::vector<OpBlock *> op_blocks;            // theirs, the graphs' and those that wait for the next user
+  cudaStream_t op_stream = nullptr;            // clears new blocks
+  unsigned long long op_calls = 0;
   cudaEvent_t ev[4] = {nullptr, nullptr, nullptr, nullptr};
 };
 
@@ -88,12 +111,21 @@ int current_device(Device **out) {
 }
 
 // Zero every stream workspace of the device (W8A8/FP16 split-K areas, the
-// opcode 2-4 stream-K scratch, the block operators' counters); the device is
-// idle when this is called.
+// opcode 2-4 stream-K scratch, the block operators' scratch, graphs' blocks
+// included); the device is idle when this is called.
+cudaError_t fill_workspaces(Device *d, int value) {
+  cudaError_t e = cudaSuccess;
+  auto fill = [&](void *base, size_t bytes) {
+    const cudaError_t r = base ? cudaMemset(base, value, bytes) : cudaSuccess;
+    if (r != cudaSuccess) e = r;
+  };
+  for (auto *m : {&d->ws, &d->qws})
+    for (auto &kv : *m) fill(kv.second.base, kv.second.bytes);
+  for (OpBlock *b : d->op_blocks) fill(b->base, b->bytes);
+  return e;
+}
 void clear_workspaces(Device *d) {
-  for (auto *m : {&d->ws, &d->qws, &d->ows})
-    for (auto &kv : *m)
-      if (kv.second.base && cudaMemset(kv.second.base, 0, kv.second.bytes) != cudaSuccess) cudaGetLastError();
+  fill_workspaces(d, 0);
   cudaDeviceSynchronize();
   cudaGetLastError();
 }
@@ -298,10 +330,7 @@ extern "C" int htpg_debug_simulate_abort(uint32_t fill) {
   int rc = current_device(&d);
   if (rc) return rc;
   if (cudaDeviceSynchronize() != cudaSuccess) return record_cuda(cudaGetLastError());
-  for (auto *m : {&d->ws, &d->qws, &d->ows})
-    for (auto &kv : *m)
-      if (kv.second.base && cudaMemset(kv.second.base, static_cast<int>(fill & 0xffu), kv.second.bytes) != cudaSuccess)
-        return record_cuda(cudaGetLastError());
+  if (fill_workspaces(d, static_cast<int>(fill & 0xffu)) != cudaSuccess) return record_cuda(cudaGetLastError());
   const uint32_t bit = 8u;  // the split-K role bit of the watchdog word
   if (cudaMemcpyToSymbol(g_watchdog, &bit, sizeof(bit)) != cudaSuccess) return record_cuda(cudaGetLastError());
   return HTPG_OK;
@@ -316,6 +345,18 @@ extern "C" int htpg_debug_workspaces(size_t *ws_bytes, size_t *qws_bytes) {
   for (auto &kv : d->qws) b += kv.second.bytes;
   if (ws_bytes) *ws_bytes = a;
   if (qws_bytes) *qws_bytes = b;
+  return HTPG_OK;
+}
+
+extern "C" int htpg_debug_op_scratch(size_t *bytes, int *blocks) {
+  Device *d;
+  int rc = current_device(&d);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lk(g_mu);
+  size_t sum = 0;
+  for (const OpBlock *b : d->op_blocks) sum += b->bytes;
+  if (bytes) *bytes = sum;
+  if (blocks) *blocks = static_cast<int>(d->op_blocks.size());
   return HTPG_OK;
 }
 
@@ -1133,40 +1174,172 @@ int op_result(cudaError_t e) { return record_cuda(e); }
 
 std::unique_lock<std::mutex> op_lock() { return std::unique_lock<std::mutex>(g_mu); }
 
-int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return HTPG_ELAUNCH;
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) return record_cuda(cudaGetLastError());
-  Workspace &w = g_dev[dev].ows[st];
-  const size_t need = kOpCounters * sizeof(uint32_t) + bytes;
-  if (w.bytes < need) {
-    if (cap != cudaStreamCaptureStatusNone) {
-      t_last_cuda_error = "the stream's scratch would have to grow during capture: run the call once before";
-      return HTPG_ENOMEM;
+namespace {
+
+// This thread may allocate while a stream of any thread is being captured.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Frees what nobody holds.  cudaFree waits for the device, and so for work of
+// streams that were destroyed with work in flight.
+void op_free_blocks(Device &d) {
+  RelaxedCapture relaxed;
+  for (size_t i = 0; i < d.op_blocks.size();) {
+    OpBlock *b = d.op_blocks[i];
+    if (b->held.load(std::memory_order_acquire) || cudaFree(b->base) != cudaSuccess) {
+      ++i;
+      continue;
     }
-    const size_t want = align_up(need + need / 4, 1u << 20);
+    d.op_blocks.erase(d.op_blocks.begin() + i);
+    delete b;
+  }
+  cudaGetLastError();
+}
+
+// A block of `need` bytes or more, its counters zero: one that was let go and is
+// not much too large, or a new one.
+int op_take(Device &d, size_t need, OpBlock **out) {
+  RelaxedCapture relaxed;
+  OpBlock *best = nullptr;
+  for (OpBlock *b : d.op_blocks)
+    if (!b->held.load(std::memory_order_acquire) && !b->dead && b->bytes >= need &&
+        b->bytes <= 4 * need + (4u << 20) && (!best || b->bytes < best->bytes))
+      best = b;
+  if (!d.op_stream && cudaStreamCreateWithFlags(&d.op_stream, cudaStreamNonBlocking) != cudaSuccess)
+    return record_cuda(cudaGetLastError());
+  if (!best) {
+    op_free_blocks(d);
+    d.op_blocks.reserve(d.op_blocks.size() + 1);
+    auto b = std::make_unique<OpBlock>();
     void *base = nullptr;
-    if (cudaMalloc(&base, want) != cudaSuccess) {
+    b->bytes = align_up(need + need / 4, 1u << 20);
+    if (cudaMalloc(&base, b->bytes) != cudaSuccess) {
       cudaGetLastError();
       return HTPG_ENOMEM;
     }
-    if (cudaMemsetAsync(base, 0, want, st) != cudaSuccess) {
-      const int rc = record_cuda(cudaGetLastError());
-      cudaFree(base);
-      return rc;
-    }
-    if (w.base && !w.captured) {
-      cudaStreamSynchronize(st);
-      cudaFree(w.base);
-    }
-    w.base = base;
-    w.bytes = want;
-    w.captured = false;
+    b->base = static_cast<uint8_t *>(base);
+    b->held = false;
+    d.op_blocks.push_back(best = b.release());
   }
-  if (cap != cudaStreamCaptureStatusNone) w.captured = true;
-  *counters = static_cast<uint32_t *>(w.base);
-  *scratch = static_cast<uint8_t *>(w.base) + kOpCounters * sizeof(uint32_t);
+  if (cudaMemsetAsync(best->base, 0, kOpCounters * sizeof(uint32_t), d.op_stream) != cudaSuccess ||
+      cudaStreamSynchronize(d.op_stream) != cudaSuccess)
+    return record_cuda(cudaGetLastError());
+  best->capture = 0;
+  best->owner = nullptr;
+  best->held = true;
+  *out = best;
+  return HTPG_OK;
+}
+
+// A stream lets go of its block, although its work may still run.
+void op_forget(Device &d, std::map<unsigned long long, OpStream>::iterator it) {
+  it->second.block->dead = true;
+  it->second.block->held = false;
+  d.ows.erase(it);
+}
+
+// Called by CUDA once the graph and its executables are gone and none runs.
+void CUDART_CB op_release(void *block) { static_cast<OpBlock *>(block)->held.store(false, std::memory_order_release); }
+
+// The block of a stream that is being captured: the graph's own, held by it and
+// by its executables, one for each stream of the capture.
+int op_graph_block(Device &d, cudaStream_t st, unsigned long long capture, cudaGraph_t graph, size_t need, OpBlock **out) {
+  static thread_local char this_thread;
+  const void *owner = st == cudaStreamPerThread ? static_cast<const void *>(&this_thread) : st;
+  for (OpBlock *b : d.op_blocks)
+    if (b->held && b->capture == capture && b->owner == owner && b->bytes >= need) {
+      *out = b;
+      return HTPG_OK;
+    }
+  OpBlock *b;
+  const int rc = op_take(d, need, &b);
+  if (rc) return rc;
+  cudaUserObject_t object;
+  cudaError_t e = cudaUserObjectCreate(&object, b, op_release, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    b->held = false;
+    return record_cuda(e);
+  }
+  e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) {
+    cudaUserObjectRelease(object, 1);  // calls op_release
+    return record_cuda(e);
+  }
+  b->capture = capture;
+  b->owner = owner;
+  *out = b;
+  return HTPG_OK;
+}
+
+// The block of a stream, by its id: handles are reused, and all threads' default
+// streams have one handle.
+int op_stream_block(Device &d, cudaStream_t st, size_t need, OpBlock **out) {
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetId(st, &id);
+  if (e != cudaSuccess) return record_cuda(e);
+  auto it = d.ows.find(id);
+  if (it != d.ows.end() && it->second.block->bytes >= need) {
+    it->second.used = ++d.op_calls;
+    *out = it->second.block;
+    return HTPG_OK;
+  }
+  if (it == d.ows.end()) {
+    // the stream that had this handle was destroyed; else, of too many, the idlest
+    auto old = d.ows.begin();
+    for (auto i = old; i != d.ows.end(); ++i) {
+      if (st != cudaStreamPerThread && i->second.handle == st) {
+        op_forget(d, i);
+        old = d.ows.end();
+        break;
+      }
+      if (i->second.used < old->second.used) old = i;
+    }
+    if (old != d.ows.end() && d.ows.size() >= kOpStreams) op_forget(d, old);
+  }
+  OpBlock *b;
+  const int rc = op_take(d, need, &b);
+  if (rc) return rc;
+  try {
+    RelaxedCapture relaxed;
+    OpStream &s = d.ows[id];
+    if (s.block) {  // outgrown: launches that use it are done before anyone else has it
+      if (cudaStreamSynchronize(st) != cudaSuccess) s.block->dead = true;
+      s.block->held = false;
+    }
+    s.handle = st;
+    s.block = b;
+    s.used = ++d.op_calls;
+  } catch (...) {
+    b->held = false;
+    throw;
+  }
+  op_free_blocks(d);
+  *out = b;
+  return HTPG_OK;
+}
+
+}  // namespace
+
+int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return HTPG_ELAUNCH;
+  Device &d = g_dev[dev];
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  cudaError_t e = cudaStreamGetCaptureInfo(st, &status, &capture, &graph);
+  if (e == cudaSuccess && status == cudaStreamCaptureStatusInvalidated) e = cudaErrorStreamCaptureInvalidated;
+  if (e != cudaSuccess) return record_cuda(e);
+  const size_t need = kOpCounters * sizeof(uint32_t) + bytes;
+  OpBlock *b;
+  const int rc = status == cudaStreamCaptureStatusActive ? op_graph_block(d, st, capture, graph, need, &b)
+                                                         : op_stream_block(d, st, need, &b);
+  if (rc) return rc;
+  *counters = reinterpret_cast<uint32_t *>(b->base);
+  *scratch = b->base + kOpCounters * sizeof(uint32_t);
   return HTPG_OK;
 }
 

@@ -31,9 +31,10 @@ int op_result(cudaError_t e);
 // so that no other host thread grows (moves) it in between.
 std::unique_lock<std::mutex> op_lock();
 // Scratch of one stream: `bytes` of it, preceded by kOpCounters zero words that
-// every launch leaves zero.  Grows when a larger call arrives (not while the
-// stream is being captured: HTPG_ENOMEM) and is kept otherwise; a block that a
-// captured graph may refer to is never freed.
+// every launch leaves zero.  Grows when a larger call arrives and is kept
+// otherwise.  While the stream is being captured it is the graph's own, so that
+// graphs run beside each other and beside the stream; with the graph and its
+// executables it goes to the next user.  Called with op_lock() held.
 constexpr int kOpCounters = 16384;
 int op_scratch(cudaStream_t st, size_t bytes, uint32_t **counters, uint8_t **scratch);
 // Tensor map of an array (any HTPG_TYPE_*) of `rank` <= 5 dimensions (innermost first;

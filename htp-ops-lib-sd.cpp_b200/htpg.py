@@ -127,6 +127,7 @@ def lib() -> ctypes.CDLL:
         "htpg_qk0_run": (I, [P, P, P, I, P]),
         "htpg_qk0_dequantize": (I, [P, P, I, I, I, P]),
         "htpg_qk0_plan_info": (I, [I, I, I, I, I, ctypes.POINTER(I64)]),
+        "htpg_debug_op_scratch": (I, [ctypes.POINTER(S), ctypes.POINTER(I)]),
         "htpg_rope_table": (I, [P, I, I, P, P]),
         "htpg_qkv_rope": (I, [P] * 12),
         "htpg_cross_attention": (I, [P] * 8),

@@ -195,6 +195,17 @@ int htpg_qk0_decode_plan_info(int weight_type, int m, int n, int k, int sms, int
 /* ---- operators of a text-conditioned transformer block -------------------
  * (no counterpart in the reference's linear path)
  *
+ * Calls go to the given stream and return before they are done.  Attention and
+ * adapters may need scratch, which the library keeps: one block per stream
+ * (a thread's cudaStreamPerThread is a stream of its own; the 128 streams that called
+ * last), which grows when a larger call arrives (HTPG_ENOMEM when it cannot), and
+ * blocks of its own for each
+ * captured graph, taken in the capture and given back with the graph and its
+ * executables.  So calls on several streams, replays of several graphs and calls
+ * on a stream that was captured may all run at once, and no call has to be made
+ * before a capture.  Two executables made from one captured graph, or graphs that
+ * contain it as a child, share its blocks: their replays have to follow one another.
+ *
  * Element types, by their ggml numbers. */
 #define HTPG_TYPE_F32 0
 #define HTPG_TYPE_F16 1
@@ -432,12 +443,16 @@ int htpg_stream_read(const void *src, size_t bytes, void *stream);
 /* Test hooks (no counterpart in the reference).  htpg_debug_simulate_abort
  * leaves, on the current device, the state a launch that gave up can leave:
  * every stream workspace (W8A8/FP16 split-K areas, opcode 2-4 stream-K
- * scratch) filled with the byte `fill` and the watchdog word set.  The next
+ * scratch, the block operators' scratch) filled with the byte `fill` and the
+ * watchdog word set.  The next
  * htpg_check_device must then answer HTPG_EWATCHDOG and restore the zeroed
  * scratch that later launches rely on.  htpg_debug_workspaces reports the
- * bytes held by the stream workspaces of the current device. */
+ * bytes held by the stream workspaces of the current device,
+ * htpg_debug_op_scratch bytes and number of the block operators' blocks,
+ * captured graphs' and free ones included. */
 int htpg_debug_simulate_abort(uint32_t fill);
 int htpg_debug_workspaces(size_t *ws_bytes, size_t *qws_bytes);
+int htpg_debug_op_scratch(size_t *bytes, int *blocks);
 
 /* Tile plan the library uses for an m x n x k problem (kind 0 = W8A8,
  * 1 = FP16) with a row-major output on a device with `sms` SMs.  out[0..11] =
