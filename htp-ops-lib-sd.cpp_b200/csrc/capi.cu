@@ -313,7 +313,9 @@ extern "C" int htpg_check_device(void *stream, uint32_t *flags) {
     // A launch that gave up may have left split-K partial sums and arrival
     // counters behind, in the W8A8/FP16 workspaces and in the opcode 2-4
     // stream-K scratch alike; both rely on "left zero by every launch".
-    // Other streams of this device may still run: wait for them first.
+    // Other streams of this device may still run: wait for them first, and let
+    // no other host thread launch or change its workspaces meanwhile.
+    std::lock_guard<std::mutex> lk(g_mu);
     cudaDeviceSynchronize();
     cudaGetLastError();
     clear_workspaces(d);
@@ -329,6 +331,7 @@ extern "C" int htpg_debug_simulate_abort(uint32_t fill) {
   Device *d;
   int rc = current_device(&d);
   if (rc) return rc;
+  std::lock_guard<std::mutex> lk(g_mu);
   if (cudaDeviceSynchronize() != cudaSuccess) return record_cuda(cudaGetLastError());
   if (fill_workspaces(d, static_cast<int>(fill & 0xffu)) != cudaSuccess) return record_cuda(cudaGetLastError());
   const uint32_t bit = 8u;  // the split-K role bit of the watchdog word
@@ -340,6 +343,7 @@ extern "C" int htpg_debug_workspaces(size_t *ws_bytes, size_t *qws_bytes) {
   Device *d;
   int rc = current_device(&d);
   if (rc) return rc;
+  std::lock_guard<std::mutex> lk(g_mu);
   size_t a = 0, b = 0;
   for (auto &kv : d->ws) a += kv.second.bytes;
   for (auto &kv : d->qws) b += kv.second.bytes;
@@ -1246,7 +1250,8 @@ void CUDART_CB op_release(void *block) { static_cast<OpBlock *>(block)->held.sto
 
 // The block of a stream that is being captured: the graph's own, held by it and
 // by its executables, one for each stream of the capture.
-int op_graph_block(Device &d, cudaStream_t st, unsigned long long capture, cudaGraph_t graph, size_t need, OpBlock **out) {
+int op_graph_block(Device &d, cudaStream_t st, unsigned long long capture, cudaGraph_t graph, size_t need,
+                   OpBlock **out) {
   static thread_local char this_thread;
   const void *owner = st == cudaStreamPerThread ? static_cast<const void *>(&this_thread) : st;
   for (OpBlock *b : d.op_blocks)
