@@ -656,6 +656,8 @@ extern "C" int htpg_lora_run(const struct htpg_lora_params *p, float *out, const
         reinterpret_cast<uintptr_t>(scales)) & 3u) ||
       (p->m > 1 && (r.ldx % 4 || r.ldo % 4 || (base && r.ldb % 4))))
     return HTPG_ECONTROL;
+  // in place a row's base is where the row goes; elsewhere another CTA may have been
+  if (p->m > 1 && base == out && r.ldb != r.ldo) return HTPG_EARGS;
   OpDevice d;
   const int rc = op_device(&d);
   if (rc) return rc;

@@ -318,8 +318,8 @@ int htpg_cross_attention(const struct htpg_attention_params *p, void *out, const
  * the first ranks[s] columns of b[s] ([adapters][n][max_rank]).  Rows whose
  * row_adapter is outside [0, adapters) get base[i].  What a and b hold past an
  * adapter's rank is not read into the result; ranks are clamped to [0,
- * max_rank].  base may be out (the projection's output, added to in place) or
- * NULL (zeros).  All of row_adapter [m], ranks and scales [adapters] (int32,
+ * max_rank].  base may be out (the projection's output, added to in place; ldb is
+ * then ldo, HTPG_EARGS otherwise) or NULL (zeros); out overlaps nothing else.  All of row_adapter [m], ranks and scales [adapters] (int32,
  * int32, FP32) are device arrays.  x, base, out FP32 with row strides ldx, ldb,
  * ldo (0: dense); a, b of `type` (F16 or BF16).  FP32 accuracy: x and the
  * intermediate x A^T are carried in parts of 22 bits or more together, and all
