@@ -1248,6 +1248,7 @@ extern "C" int htpg_cross_attention(const struct htpg_attention_params *p, void 
       !(p->scale > 0.0f) || !std::isfinite(p->scale))
     return HTPG_EARGS;
   if (p->q_heads % p->kv_heads || p->head_dim % 8 || p->head_dim > kAttnMaxDim) return HTPG_ECAPACITY;
+  if (std::max(p->q_len, p->kv_len) > kOpMaxExtent) return HTPG_ECAPACITY;
   if (p->batch == 0 || p->q_len == 0) return HTPG_OK;
   if (!out || !q || (p->kv_len && (!k || !v))) return HTPG_EARGS;
   const int qe[3] = {p->batch, p->q_len, p->q_heads}, ke[3] = {p->batch, p->kv_len, p->kv_heads};

@@ -643,6 +643,7 @@ extern "C" int htpg_lora_run(const struct htpg_lora_params *p, float *out, const
       p->adapters < 1 || p->max_rank < 1 || p->ldx < 0 || p->ldb < 0 || p->ldo < 0)
     return HTPG_EARGS;
   if (p->k % 8 || p->n % 8 || p->max_rank % 8 || p->max_rank > kLoraMaxRank) return HTPG_ECAPACITY;
+  if (std::max({p->m, p->k, p->n}) > kOpMaxExtent) return HTPG_ECAPACITY;
   if (p->m == 0) return HTPG_OK;
   if (!out || !x || !row_adapter || !a || !b || !ranks || !scales) return HTPG_EARGS;
   LoraArgs r = {};

@@ -59,6 +59,9 @@ cudaError_t op_launch(void (*fn)(P...), dim3 grid, unsigned block, size_t smem, 
   return counted(cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...));
 }
 
+// Extents up to this one can be rounded up to tiles, and passed by a step, in 32 bits.
+constexpr int kOpMaxExtent = 1 << 30;
+
 // ---- element types
 inline int type_bytes(int type) {
   return type == HTPG_TYPE_F32 ? 4 : type == HTPG_TYPE_F16 || type == HTPG_TYPE_BF16 ? 2 : 0;

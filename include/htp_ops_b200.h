@@ -298,8 +298,8 @@ int htpg_qkv_rope(const struct htpg_rope_params *p, void *q_out, void *k_out, vo
  * 192; q_heads a multiple of kv_heads; scale > 0.  Pointers 16-byte aligned
  * (kv_lens, key_bias: 4); along dimensions longer than one, strides are
  * multiples of 8 elements (out: of 16 bytes), below 2^38, not negative, and not
- * zero for tokens and in out (HTPG_ECONTROL).  batch or q_len 0: nothing is
- * done; kv_len 0: zeros. */
+ * zero for tokens and in out (HTPG_ECONTROL).  q_len, kv_len up to 2^30.  batch or
+ * q_len 0: nothing is done; kv_len 0: zeros. */
 struct htpg_attention_params {
   int32_t type, out_type; /* HTPG_TYPE_* */
   int32_t batch, q_len, kv_len;
@@ -324,8 +324,9 @@ int htpg_cross_attention(const struct htpg_attention_params *p, void *out, const
  * ldo (0: dense); a, b of `type` (F16 or BF16).  FP32 accuracy: x and the
  * intermediate x A^T are carried in parts of 22 bits or more together, and all
  * sums are FP32.
- * k, n: multiples of 8; max_rank: a multiple of 8 up to 128; pointers 16-byte
- * aligned, ld* multiples of 4 (HTPG_ECONTROL).  m = 0: nothing is done. */
+ * m, k, n up to 2^30; k, n: multiples of 8; max_rank: a multiple of 8 up to 128;
+ * pointers 16-byte aligned, ld* multiples of 4 (HTPG_ECONTROL).  m = 0: nothing is
+ * done. */
 struct htpg_lora_params {
   int32_t type; /* of a and b */
   int32_t m, k, n;

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 import htpg
-from test_block_operators import A16, LORA
+from test_block_operators import A16, LORA, _attn
 
 
 def lora(lib, **change):
@@ -20,3 +20,22 @@ def test_lora_base_in_place_has_the_output_rows(lib):
     assert lora(lib, ldb=96, ldo=104) == htpg.EARGS
     assert lora(lib, ldb=104, ldo=96) == htpg.EARGS
     assert lora(lib, ldb=0, ldo=104) == htpg.EARGS      # dense base
+
+
+BIG = 2**31 - 1
+
+
+@pytest.mark.parametrize("name", ["m", "k", "n"])
+def test_lora_sizes_whose_index_arithmetic_would_wrap(lib, name):
+    """Sizes are rounded up to whole tiles in 32 bits."""
+    dense = dict(ldx=0, ldb=0, ldo=0)
+    for size in ((BIG, 2**30 + 1) if name == "m" else (BIG - 7, 2**30 + 8)):
+        assert lora(lib, **dense, **{name: size}) == htpg.ECAPACITY
+
+
+@pytest.mark.parametrize("name", ["q_len", "kv_len"])
+def test_attention_lengths_whose_index_arithmetic_would_wrap(lib, name):
+    for size in (BIG, 2**30 + 1):
+        p = _attn(**{name: size})
+        args = dict.fromkeys(("out", "q", "k", "v"), A16)
+        assert lib.htpg_cross_attention(ctypes.byref(p), *args.values(), None, None, None) == htpg.ECAPACITY
