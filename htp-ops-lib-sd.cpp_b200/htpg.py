@@ -207,11 +207,12 @@ def _current_raw_stream() -> int:
     """torch's current stream of the current device (0.4 us where building a torch.cuda.Stream takes 3.5)."""
     global _current_raw_stream
     import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is None:
+    raw, device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
+    if raw is None or device is None:
         _current_raw_stream = lambda: torch.cuda.current_stream().cuda_stream
     else:
-        _current_raw_stream = lambda: raw(torch.cuda.current_device())
+        torch.cuda.current_device()  # initialises CUDA
+        _current_raw_stream = lambda: raw(device())
     return _current_raw_stream()
 
 
@@ -515,20 +516,16 @@ def _dptr(t) -> int | None:
     raise ValueError("a tensor in pageable host memory")
 
 
-def _array(t, name: str, dtype, n: int) -> int | None:
+def _array(t, name: str, dtype, n: int) -> int:
     """Address of an array of a call: dense, at least n elements of one type (the library sees the address alone)."""
-    if t is None:
-        return None
     if t.dtype is dtype and t.numel() >= n and t.is_contiguous():
         return t.data_ptr() if t.is_cuda else _dptr(t)
     raise ValueError(f"{name}: expected a dense {dtype} array of {n} elements or more, got {tuple(t.shape)}, strides "
                      f"{t.stride()}, {t.dtype}")
 
 
-def _bias(t, prm) -> int | None:
+def _bias(t, prm) -> int:
     """Address of a key bias: FP32, prm.batch rows of prm.kv_len elements, prm.bias_stride apart."""
-    if t is None:
-        return None
     import torch
     step, keys, shape = prm.bias_stride, prm.kv_len, t.shape
     reach = (prm.batch - 1) * step + keys  # elements from the first to the last that are read
@@ -578,10 +575,12 @@ def qkv_rope(prm: RopeParams, q_out, k_out, v_out, q, k, v, q_weight=None, k_wei
     """Weights FP32 [dim], table FP32 [table_rows][rot_dim / 2][2], positions int32 [batch][seq]: dense."""
     import torch
     f32, dim = torch.float32, prm.head_dim
-    return lib().htpg_qkv_rope(ctypes.byref(prm), _dptr(q_out), _dptr(k_out), _dptr(v_out), _dptr(q), _dptr(k), _dptr(v),
-                               _array(q_weight, "q_weight", f32, dim), _array(k_weight, "k_weight", f32, dim),
-                               _array(table, "table", f32, prm.table_rows * prm.rot_dim),
-                               _array(positions, "positions", torch.int32, prm.batch * prm.seq), stream_ptr(stream))
+    qw = None if q_weight is None else _array(q_weight, "q_weight", f32, dim)
+    kw = None if k_weight is None else _array(k_weight, "k_weight", f32, dim)
+    at = None if table is None else _array(table, "table", f32, prm.table_rows * prm.rot_dim)
+    pos = None if positions is None else _array(positions, "positions", torch.int32, prm.batch * prm.seq)
+    return lib().htpg_qkv_rope(ctypes.byref(prm), _dptr(q_out), _dptr(k_out), _dptr(v_out), _dptr(q), _dptr(k),
+                               _dptr(v), qw, kw, at, pos, stream_ptr(stream))
 
 
 def attention_params(out, q, k, v, scale: float, bias_stride: int | None = None) -> AttentionParams:
@@ -601,8 +600,9 @@ def attention_params(out, q, k, v, scale: float, bias_stride: int | None = None)
 def cross_attention(prm: AttentionParams, out, q, k, v, kv_lens=None, key_bias=None, stream=None) -> int:
     """kv_lens: int32 [batch], dense; key_bias: FP32, rows of kv_len elements prm.bias_stride apart."""
     import torch
-    return lib().htpg_cross_attention(ctypes.byref(prm), _dptr(out), _dptr(q), _dptr(k), _dptr(v),
-                                      _array(kv_lens, "kv_lens", torch.int32, prm.batch), _bias(key_bias, prm),
+    lens = None if kv_lens is None else _array(kv_lens, "kv_lens", torch.int32, prm.batch)
+    bias = None if key_bias is None else _bias(key_bias, prm)
+    return lib().htpg_cross_attention(ctypes.byref(prm), _dptr(out), _dptr(q), _dptr(k), _dptr(v), lens, bias,
                                       stream_ptr(stream))
 
 
