@@ -10,7 +10,8 @@
 
 Every request of the batch has its own text length and its own adapter (or
 none).  All calls go to the current stream and allocate nothing after the first
-one, so the block can be captured in a CUDA graph (done here for the timing)."""
+one there, so the block can be captured in a CUDA graph (done here for the timing;
+the graph takes scratch of its own for attention and adapters)."""
 import os
 import sys
 

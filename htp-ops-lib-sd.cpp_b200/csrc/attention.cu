@@ -44,16 +44,20 @@ struct AttnArgs {
 // ([key][dim]), the MN-major B operand.
 // Rounding: scores and sums are FP32; the weights are rounded to the 16 bits of
 // the tensor core's A operand (with FP32 outputs the rest follows as a second
-// operand), the sum they are divided by is of the unrounded ones.  The maximum is
+// operand), the sum they are divided by is of the unrounded ones.  16-bit outputs
+// are then off by a third more than the exact result rounded once (0.00028 against
+// 0.00021 of the norm, FP16); the second operand would take that away for the time
+// that FP32 outputs show below.  The maximum is
 // only raised (and O rescaled) once a score passes it by 2^kLazy, which changes
 // no weight's relative error and lets most tiles skip the rescale.
-// Bound by the issue of the softmax's instructions and the latency of one step's
-// chain, not by the tensor core: 4 x 4096 queries of 12 heads of 128 over 4096
-// keys, FP16: 407 us = 1010 TFLOP/s (0.61 of cuBLAS); 16384 over 512, BF16: 81 us.
-// 64 keys a tile: 128 with one buffer of S 611 us.  Turns at the exponentials 489
-// -> 455, one elected lane issuing 548 -> 489.  Few keys are bound by an item's
-// chain load -> scores -> weights -> output, about 3.5 us: 2 x 4096 queries of 24
-// heads of 64 over 77 keys 28.6 us.
+// Bound by the latency of one step's chain, with no unit full (tensor pipe 34 %,
+// issue slots 37 %).  Times alone (the call repeated in a graph): 4 x 4096 queries
+// of 12 heads of 128 over 4096 keys, FP16: 407 us = 1010 TFLOP/s (0.61 of cuBLAS)
+// for ten after a pause, 457 to 468 kept up, where the power cap lowers the clocks;
+// 16384 over 512, BF16: 79 us.  64 keys a tile: 128 with one buffer of S 611 us.
+// Turns at the exponentials 489 -> 455, one elected lane issuing 548 -> 489.  Few
+// keys are bound by an item's chain load -> scores -> weights -> output, about
+// 3.5 us: 2 x 4096 queries of 24 heads of 64 over 77 keys 27.5 us (FP32 out 29.3).
 constexpr int kTileThreads = 384;
 constexpr int kLensHeld = 256;   // batches whose lengths are kept in shared memory
 constexpr float kLazy = 8.0f;    // log2 of how far a score may pass the held maximum
@@ -108,8 +112,9 @@ constexpr bool tile_staged(int dp) {
 // per CTA and tile, and begins anew. Four tiles keep the loss below what FP32
 // sums over thousands of keys lose anyway: 4096 queries over 4096 keys of 128,
 // error 5.2e-6 without, 1.7e-6 with eight, 1.1e-6 with four (FP32 products summed
-// in order: 1.4e-6). The sums stay in L2; four floats per atomic, 530 us
-// (one per atomic 677).
+// in order: 1.4e-6). The sums stay in L2; four floats per atomic: 2 x 4096 queries
+// of 12 heads of 128 over 4096 keys 530 us (one per atomic 677); of 24 heads of 64
+// 609, where 16-bit outputs take 378.
 constexpr int kFlush = 4;
 
 struct TileItem {
@@ -730,9 +735,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 // memory, and over the key ranges of a unit by its last CTA, in order.  Keys
 // that take no part are never copied: their rows are zeros.  Weights are rounded
 // as in the tiles above (two parts for FP32 outputs).
-// 16 requests, 32 heads in 8 groups of 128, over 1500 keys and fewer: 22 us for
-// 74 MB (3.4 TB/s; the wave's tail and the chain copy -> scores -> weights of each
-// warp's chunks, 25 % issue); one request over 8192 keys: 13 us for 34 MB.
+// 16 requests, 32 heads in 8 groups of 128, over 1500 keys and fewer, FP32 out: 22 us
+// for 74 MB with K and V in part in L2, 28.6 in a sequence of calls on other ones (2.6
+// TB/s; the wave's tail and the chain copy -> scores -> weights of each warp's
+// chunks, 25 % issue); one request over 8192 keys: 13 us for 34 MB.
 constexpr int kFewWarps = 4, kFewRows = 16, kFewKeys = 16;
 
 struct FewArgs {

@@ -302,8 +302,9 @@ struct UpSmem {
 // kDepth blocks (16 rows x 32 columns) of base in flight in a ring of its own, read
 // back by the lanes that copied them.
 // Many rows: bound by L1 and the chain of an item, then HBM (16384 rows x 6144, rank
-// 64: 169 us for 805 MB, L1 78 % busy; both passes 208 us in a sequence); few rows
-// by the chain ids -> t -> out (one row, both passes: 8 us).
+// 64: 169 us under ncu for 805 MB, L1 78 % busy; both passes 211 to 216 us alone, 228
+// in a sequence of calls on other rows); few rows by the chain ids -> t -> out (one
+// row, both passes: 8 us).
 template <typename T, int RK>
 __global__ void __launch_bounds__(kLoraThreads, 2)
     lora_up_kernel(const __grid_constant__ LoraArgs p, const float *part, int ranges, int n_range) {
@@ -506,7 +507,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       take(next, z + at * zs, group);
     copy_wait<D - 1>();
     if (rank == 0 && in_place) continue;
-    // base joins after the products: 16 registers fewer next to B (rank 128: 210 -> 190 us)
+    // base joins after the products: 16 registers fewer next to B (16384 x 1536 x 1536, rank
+    // 128: 210 -> 190 us)
     float acc[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
@@ -567,7 +569,8 @@ int launch_lora(const LoraArgs &p, const OpDevice &d, cudaStream_t st) {
   // two CTAs per SM 23.9), then a tile's blocks side by side.  Tiles of 32 or, up
   // to rank 64, 128 rows, whichever takes fewer rounds of (rows x elements + a CTA's
   // set-up, about as long as 32 rows x 1024 elements): 16384 x 1536 x 6144, rank 64:
-  // 226 us in all with 32, 216 with 128; mixed, rank 16: 269, 247; rank 128: 210, 215.
+  // 226 us in all with 32, 216 with 128; mixed, rank 16: 269, 247; 16384 x 1536 x 1536,
+  // rank 128: 210, 215.
   struct Plan {
     int tiles, k_range, k_ranges;
     long long cost;

@@ -61,7 +61,7 @@ constexpr int kRopeWarps = 8, kRopeMaxDim = 512;
 
 // Any size and alignment (odd head dims, rotations that are no multiple of 4):
 // one warp per (token, head) row, the row staged in shared memory as FP32.  Bound
-// by latency: 16384 tokens of 24 heads of 70, FP32 to FP16: 195 us (heads of 72,
+// by latency: 16384 tokens of 24 heads of 70, FP32 to FP16: 186 us (heads of 72,
 // in vectors: 51).
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_row_kernel(RopeArgs a) {

@@ -294,7 +294,10 @@ int htpg_qkv_rope(const struct htpg_rope_params *p, void *q_out, void *k_out, vo
  * v); out_type: the same or F32.  The weights are rounded to `type` for the
  * product with V; with an F32 output they are carried in two parts (twice the
  * bits) and summed in FP32, so that the result is good to a few 2^-20 (F16) or
- * to about 2^-16 (BF16) of the largest value.  head_dim: a multiple of 8 up to
+ * to about 2^-16 (BF16) of the largest value, and to what FP32 scores leave: a
+ * weight is off by a few 2^-23 times the sizes added up in its score, sum |q_d k_d|
+ * scale + |bias|.  Infinities of keys that take part, in V or in a score, may
+ * give NaN where the formula gives an infinity.  out overlaps no input.  head_dim: a multiple of 8 up to
  * 192; q_heads a multiple of kv_heads; scale > 0.  Pointers 16-byte aligned
  * (kv_lens, key_bias: 4); along dimensions longer than one, strides are
  * multiples of 8 elements (out: of 16 bytes), below 2^38, not negative, and not
@@ -323,7 +326,8 @@ int htpg_cross_attention(const struct htpg_attention_params *p, void *out, const
  * int32, FP32) are device arrays.  x, base, out FP32 with row strides ldx, ldb,
  * ldo (0: dense); a, b of `type` (F16 or BF16).  FP32 accuracy: x and the
  * intermediate x A^T are carried in parts of 22 bits or more together, and all
- * sums are FP32.
+ * sums are FP32.  An infinity in x, a or b may give NaN where the formula gives an
+ * infinity.
  * m, k, n up to 2^30; k, n: multiples of 8; max_rank: a multiple of 8 up to 128;
  * pointers 16-byte aligned, ld* multiples of 4 (HTPG_ECONTROL).  m = 0: nothing is
  * done. */
