@@ -205,6 +205,7 @@ int htpg_qk0_decode_plan_info(int weight_type, int m, int n, int k, int sms, int
  * on a stream that was captured may all run at once, and no call has to be made
  * before a capture.  Two executables made from one captured graph, or graphs that
  * contain it as a child, share its blocks: their replays have to follow one another.
+ * A graph that an executable was updated from has to outlive it.
  *
  * Element types, by their ggml numbers. */
 #define HTPG_TYPE_F32 0
