@@ -196,12 +196,11 @@ int htpg_qk0_decode_plan_info(int weight_type, int m, int n, int k, int sms, int
  * (no counterpart in the reference's linear path)
  *
  * Calls go to the given stream and return before they are done.  Attention and
- * adapters may need scratch, which the library keeps: one block per stream
- * (a thread's cudaStreamPerThread is a stream of its own; the 128 streams that called
- * last), which grows when a larger call arrives (HTPG_ENOMEM when it cannot), and
- * blocks of its own for each
- * captured graph, taken in the capture and given back with the graph and its
- * executables.  So calls on several streams, replays of several graphs and calls
+ * adapters may need scratch, which the library keeps: one block for each of the 128
+ * streams that called last (a thread's cudaStreamPerThread is a stream of its own),
+ * which grows when a larger call arrives (HTPG_ENOMEM when it cannot), and blocks
+ * of its own for each captured graph, taken in the capture and given back with the
+ * graph and its executables.  So calls on several streams, replays of several graphs and calls
  * on a stream that was captured may all run at once, and no call has to be made
  * before a capture.  Two executables made from one captured graph, or graphs that
  * contain it as a child, share its blocks: their replays have to follow one another.
